@@ -1,0 +1,73 @@
+"""LayerNorm without an activation, for rows in fp32, bf16 or fp16 (``nn.LayerNorm(E)``; the world model's blocks use the form fused
+with SiLU, lib/world_model.py:153-160).
+
+``layer_norm`` is one kernel forward and two backward (the row pass, which also forms the column sums of the weight's and the
+bias's gradient, and their sum over workgroups).  Statistics and sums are fp32 whatever the rows' type; results are rounded once.
+Host tensors take the formula in tensor operations.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _native as N
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        rows = N.as_rows(x)
+        stats = any(ctx.needs_input_grad[:3])
+        y, mean, rstd = N.layer_norm_forward(rows, weight, bias, eps, stats)
+        if stats:
+            ctx.save_for_backward(rows, weight, mean, rstd)
+            ctx.bias_dtype = None if bias is None else bias.dtype
+        return y.view(x.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        rows, weight, mean, rstd = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = N.layer_norm_backward(rows, N.as_rows(dy), weight, mean, rstd, need[0], weight.dtype if need[1] else None,
+                                           ctx.bias_dtype if need[2] else None)
+        return None if dx is None else dx.view(dy.shape), dw, db, None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x (any leading shape; rows may be strided).
+
+    x in fp32, bf16 or fp16; weight and bias (E,) in fp32 or in x's type, or None.  The result is dense, in x's type, and
+    differentiable with respect to x, weight and bias (once)."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise N.NativeError(f"layer_norm: rows of at least one element, got shape {tuple(x.shape)}")
+    if x.is_cuda:
+        return _LayerNormFn.apply(x, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), float(eps))
+    N.dtype_id(x, "x")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.shape != x.shape[-1:] or t.dtype not in (torch.float32, x.dtype) or t.device != x.device):
+            raise N.NativeError(f"layer_norm: {name} {tuple(t.shape)} {t.dtype} on {t.device} does not fit rows {tuple(x.shape)} {x.dtype}")
+    v = x.float()
+    c = v - v.mean(-1, keepdim=True)
+    y = c * torch.rsqrt(c.square().mean(-1, keepdim=True) + eps)
+    y = y if weight is None else y * weight.float()
+    return (y if bias is None else y + bias.float()).to(x.dtype)
+
+
+class LayerNorm(nn.LayerNorm):
+    """``nn.LayerNorm`` over the last dimension (same parameters and state-dict keys) on ``layer_norm``; parameters may stay in
+    fp32 while the rows are bf16 or fp16."""
+
+    def __init__(self, normalized_shape, eps: float = 1e-5, elementwise_affine: bool = True, bias: bool = True, device=None, dtype=None):
+        super().__init__(normalized_shape, eps, elementwise_affine, bias, device, dtype)
+        if len(self.normalized_shape) != 1:
+            raise ValueError(f"LayerNorm normalises the last dimension only, got normalized_shape={tuple(self.normalized_shape)}")
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.shape[-1:] != tuple(self.normalized_shape):
+            raise ValueError(f"LayerNorm over {self.normalized_shape[0]} elements got rows of {x.shape[-1] if x.dim() else 0}")
+        return layer_norm(x, self.weight, self.bias, self.eps)

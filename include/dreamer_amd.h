@@ -39,6 +39,11 @@ extern "C" {
 
 #define DRM_MAX_MLP_LAYERS 4
 
+/* element types of the operators that take more than fp32 */
+#define DRM_F32 0
+#define DRM_BF16 1
+#define DRM_F16 2
+
 typedef void* drm_stream_t; /* hipStream_t */
 
 /* ---- library ------------------------------------------------------------------------------ */
@@ -518,6 +523,67 @@ int drm_ln_silu_backward(const float* x, const float* dy, const float* gamma, co
                          const float* rstd, float* dx, float* param_partials, int64_t N, int32_t E,
                          const float* channel_bias, int32_t hw, int32_t channels_last, float* sample_sums,
                          drm_stream_t stream);
+
+/* ---- LayerNorm over the rows of a matrix (nn.LayerNorm(E), no activation), forward and backward -------------------------
+ * x, dy: (N, E) with row strides ldx, lddy >= E (elements; columns contiguous), fp32, bf16 or fp16 (x_dtype), aligned to their
+ * own element only.  w, b: (E) or NULL (1 / 0), w_dtype = DRM_F32 or x_dtype.  Statistics and sums are fp32, results are rounded
+ * once to their type.
+ *   forward : y (N, E; row stride ldy) = (x - mean) * rstd * w + b; mean, rstd (N, fp32) are written when not NULL (both or
+ *             neither).
+ *   backward: dx (N, E; dense, x_dtype), dw, db (E; w_dtype), each of them optional.  dw and db are summed over the rows through
+ *             `workspace` (drm_layer_norm_workspace_bytes(N, E)) in an order that depends on N and E only.
+ * N = 0 is allowed (dw = db = 0). */
+int drm_layer_norm_forward(const void* x, int64_t ldx, int32_t x_dtype, const void* w, const void* b, int32_t w_dtype, void* y,
+                           int64_t ldy, float* mean, float* rstd, int64_t N, int32_t E, float eps, drm_stream_t stream);
+size_t drm_layer_norm_workspace_bytes(int64_t N, int32_t E);
+int drm_layer_norm_backward(const void* x, int64_t ldx, const void* dy, int64_t lddy, int32_t x_dtype, const void* w, int32_t w_dtype,
+                            const float* mean, const float* rstd, void* dx, void* dw, void* db, int64_t N, int32_t E, void* workspace,
+                            size_t workspace_bytes, drm_stream_t stream);
+
+/* ---- distillation from a teacher's top logits ----------------------------------------------------------------------------
+ * logits: (rows, V) student logits, row stride ld_logits, fp32 / bf16 / fp16; q = softmax(logits / temperature).  The teacher is a
+ * list per row: top_values (rows, k) fp32 logits at top_indices (rows, k), row strides ld_values, ld_indices; k <= 1024.  Entries whose
+ * index is outside [0, V) are absent; a row without entries (or whose values are all -inf, without top_lse) has loss 0 and gradient 0.
+ *   top_lse == NULL: p_j = softmax over the listed values / temperature;
+ *   top_lse (rows) : log-sum-exp of the teacher's whole row of logits / temperature; p_j = exp(value / temperature - top_lse), and the
+ *                    rest P = max(0, 1 - sum p) is held against the student's mass outside the list, Q (left out where that is 0).
+ *   loss[r] = sum_j p_j (log p_j - log q_{i_j}) + P (log P - log Q)
+ * forward also writes p_out (rows, k) and row_out (rows, 4), which backward takes; `workspace`:
+ * drm_distill_topk_workspace_bytes(rows, V) bytes (may be 0).  backward: d_logits (rows, V; dense, the logits' type) =
+ * g_rows[r] * d loss[r] / d logits.  An index that is listed more than once counts with each of its p_j. */
+size_t drm_distill_topk_workspace_bytes(int64_t rows, int32_t V);
+int drm_distill_topk_forward(const void* logits, int64_t ld_logits, int32_t dtype, const float* top_values, int64_t ld_values,
+                             const int64_t* top_indices, int64_t ld_indices, const float* top_lse, int64_t rows, int32_t V, int32_t k,
+                             double temperature, float* loss, float* p_out, float* row_out, void* workspace, size_t workspace_bytes,
+                             drm_stream_t stream);
+int drm_distill_topk_backward(const void* logits, int64_t ld_logits, int32_t dtype, const int64_t* top_indices, int64_t ld_indices,
+                              const float* p, const float* row, const float* g_rows, int64_t rows, int32_t V, int32_t k,
+                              double temperature, void* d_logits, drm_stream_t stream);
+
+/* ---- microscaled 4-bit matrices --------------------------------------------------------------------------------------------
+ * A matrix (rows, K) in blocks of 32 along its rows, nb = ceil(K / 32): codes (rows, nb, 16 bytes), e2m1 with element 2i of the block in
+ * the low half of byte i, and scales (rows, nb), one byte s per block standing for 2^(s - 127), 255 for a block of NaN.  Both dense,
+ * codes 16-byte aligned; codes behind column K are 0.
+ *   quantize  : s - 127 = floor(log2(max |x|)) - 2 clamped to [-127, 127]; codes = x / 2^(s-127) to the nearest of 0, 0.5, 1, 1.5, 2, 3,
+ *               4, 6 (ties to the even code), 6 beyond; a block with an infinity or NaN gets s = 255.
+ *   linear    : y (M, N) = x W^T + bias with x (M, K) in fp32 / bf16 / fp16 (y the same type; bias any of them or NULL): the products
+ *               are exact (x in bf16 parts on the bf16 matrix pipe), sums are fp32.
+ *   dgrad     : dx (M, K) = dy W, the input gradient of `linear`.
+ *   product   : y (M, N) = X W^T + bias with both operands in 4 bits (scaled matrix instructions), y of y_dtype. */
+int drm_mx4_quantize(const void* x, int64_t ldx, int32_t dtype, int64_t rows, int32_t K, uint8_t* codes, uint8_t* scales,
+                     drm_stream_t stream);
+int drm_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int32_t K, void* y, int64_t ldy, int32_t dtype,
+                       drm_stream_t stream);
+int drm_mx4_linear(const void* x, int64_t ldx, int32_t dtype, const uint8_t* codes, const uint8_t* scales, const void* bias,
+                   int32_t bias_dtype, void* y, int64_t ldy, int32_t M, int32_t N, int32_t K, drm_stream_t stream);
+int drm_mx4_linear_dgrad(const void* dy, int64_t lddy, int32_t dtype, const uint8_t* codes, const uint8_t* scales, void* dx,
+                         int64_t lddx, int32_t M, int32_t N, int32_t K, drm_stream_t stream);
+/* bias gradient of `linear`: column sums of dy (M, N) in db_dtype, added in fp32 in an order that depends on M and N only */
+size_t drm_mx4_bias_grad_workspace_bytes(int32_t M, int32_t N);
+int drm_mx4_bias_grad(const void* dy, int64_t lddy, int32_t dtype, void* db, int32_t db_dtype, int32_t M, int32_t N, void* workspace,
+                      size_t workspace_bytes, drm_stream_t stream);
+int drm_mx4_product(const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales, const void* bias,
+                    int32_t bias_dtype, void* y, int64_t ldy, int32_t y_dtype, int32_t M, int32_t N, int32_t K, drm_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,334 @@
+"""Microscaled 4-bit matrices: quantisation against the definition, products against 64 bits."""
+import pytest
+import torch
+
+from dreamer_amd import _native as N
+from dreamer_amd import mx4
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def quantise(x):
+    """codes (rows, nb * 16), scales (rows, nb) and values of a float matrix, in 64 bits on the host, by distance to the levels."""
+    x = x.detach().double().cpu()
+    rows, K = x.shape
+    nb = -(-K // 32)
+    v = torch.zeros(rows, nb * 32, dtype=torch.float64)
+    v[:, :K] = x
+    v = v.view(rows, nb, 32)
+    top = v.abs().amax(2)
+    bad = ~torch.isfinite(v).all(2)
+    e = torch.full((rows, nb), -127.0, dtype=torch.float64)
+    live = (top > 0) & ~bad
+    e[live] = (torch.frexp(top[live])[1].double() - 3).clamp(-127, 127)
+    unit = torch.pow(torch.tensor(2.0, dtype=torch.float64), e)
+    a = (v.abs() / unit.unsqueeze(2)).clamp_max(6.0)
+    levels = torch.tensor(LEVELS, dtype=torch.float64)
+    near = (a.unsqueeze(-1) - levels).abs()
+    best = near.amin(-1, keepdim=True)
+    hit = near == best
+    even = hit & (torch.arange(8) % 2 == 0)
+    code = torch.where(even.any(-1), even.double().argmax(-1), hit.double().argmax(-1))
+    code[bad] = 0
+    values = torch.where(torch.signbit(v), -levels[code], levels[code]) * unit.unsqueeze(2)
+    values[bad] = float("nan")
+    sign = torch.signbit(v) & ~bad.unsqueeze(2)
+    code = code + 8 * sign
+    packed = (code[:, :, 0::2] + 16 * code[:, :, 1::2]).to(torch.uint8).reshape(rows, nb * 16)
+    scales = torch.where(bad, torch.full_like(e, 255.0), e + 127).to(torch.uint8)
+    return packed, scales, values.reshape(rows, nb * 32)[:, :K]
+
+
+def weight(rows, K, seed=0, scale=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed + rows + K)
+    return mx4.quantize(torch.randn(rows, K, generator=g, device=DEV) * scale)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,K", [(1, 1), (3, 31), (5, 32), (2, 33), (7, 100), (130, 64), (33, 4080), (1, 8191)])
+def test_quantise_and_back(rows, K, dtype):
+    g = torch.Generator(device=DEV).manual_seed(rows * K)
+    x = (torch.randn(rows, K, generator=g, device=DEV) * torch.exp2(torch.randint(-9, 9, (rows, 1), generator=g, device=DEV).float())).to(dtype)
+    q = mx4.quantize(x)
+    codes, scales, values = quantise(x)
+    assert torch.equal(q.scales.cpu(), scales) and torch.equal(q.codes.cpu(), codes)
+    assert q.shape == (rows, K)
+    for t in (F32, BF16, F16):
+        assert torch.equal(q.dequantize(t).cpu(), values.to(t)), t
+
+
+def test_every_code_tie_and_scale():
+    # each tie, its neighbours on both sides, saturation, signs, at scales over the whole range of fp32
+    mids = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 0.0])
+    pts = torch.cat([mids, torch.nextafter(mids, torch.tensor(0.0)), torch.nextafter(mids, torch.tensor(99.0))])
+    block = torch.zeros(32)
+    block[:30] = pts * torch.where(torch.arange(30) % 2 == 0, 1.0, -1.0)
+    block[30], block[31] = 4.0, -0.0
+    exps = torch.tensor([-120.0, -60.0, -1.0, 0.0, 1.0, 60.0, 120.0])
+    x = (block.unsqueeze(0) * torch.exp2(exps).unsqueeze(1)).to(DEV)
+    q = mx4.quantize(x)
+    codes, scales, values = quantise(x)
+    assert torch.equal(q.scales.cpu(), scales) and torch.equal(q.codes.cpu(), codes) and torch.equal(q.dequantize().cpu(), values.float())
+
+
+def test_zero_tiny_huge_and_special_blocks():
+    x = torch.zeros(8, 64, device=DEV)
+    x[0, 32:] = 2.0 ** -149
+    x[1, :32] = 2.0 ** -126
+    x[2] = torch.finfo(F32).max
+    x[3, 5] = float("nan")
+    x[4, 40] = float("inf")
+    x[5, 3] = float("-inf")
+    x[6, :] = -0.0
+    x[7, 0], x[7, 1], x[7, 2] = 6 * 2.0 ** -127, 2.0 ** -128, 3 * 2.0 ** -129
+    q = mx4.quantize(x)
+    codes, scales, values = quantise(x)
+    assert torch.equal(q.scales.cpu(), scales) and torch.equal(q.codes.cpu(), codes)
+    y = q.dequantize().cpu()
+    assert torch.equal(torch.isnan(y), torch.isnan(values)) and torch.equal(torch.nan_to_num(y, 0.0), torch.nan_to_num(values.float(), 0.0))
+
+
+def test_every_scale_byte_dequantises():
+    codes = torch.randint(0, 256, (1, 16 * 256), dtype=torch.uint8, device=DEV)
+    scales = torch.arange(256, dtype=torch.uint8, device=DEV).view(1, 256)
+    y = mx4.MX4Tensor(codes, scales, 256 * 32).dequantize().cpu().view(256, 32)
+    c = codes.cpu().view(256, 16).long()
+    nib = torch.stack([c & 15, c >> 4], 2).view(256, 32)
+    lev = torch.tensor(LEVELS, dtype=torch.float64)
+    v = torch.where(nib >= 8, -lev[nib & 7], lev[nib & 7]) * torch.pow(torch.tensor(2.0, dtype=torch.float64), torch.arange(256).double() - 127).unsqueeze(1)
+    assert torch.isnan(y[255]).all() and torch.equal(y[:255], v[:255].float())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_quantise_strided_rows_and_leading_dimensions(dtype):
+    full = torch.randn(9, 107, device=DEV).to(dtype)
+    a, b = mx4.quantize(full[:, 3:70]), mx4.quantize(full[:, 3:70].contiguous())
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+    c = mx4.quantize(full[:, 3:70].contiguous().view(3, 3, 67))
+    assert torch.equal(c.codes, b.codes) and c.shape == (9, 67)
+    z = mx4.quantize(torch.zeros(0, 40, device=DEV, dtype=dtype))
+    assert z.shape == (0, 40) and z.dequantize().shape == (0, 40)
+
+
+def _bound(x, w, b, y, K, parts, dtype):
+    """Half a step of the result's type; sums of `parts` * K products (exact) in fp32: at most that many half steps of the sum of their
+    magnitudes, and one more for the bias."""
+    mag = x.abs() @ w.abs().t()
+    return torch.finfo(dtype).eps / 2 * y.abs() + (parts * K + 2) * U * (mag + (0 if b is None else b.double().abs())) \
+        + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+
+
+PARTS = {F32: 3, BF16: 1, F16: 2}
+SHAPES = [(1, 1, 1), (1, 16, 32), (2, 17, 33), (15, 40, 100), (16, 1000, 512), (17, 31, 96), (33, 130, 257), (64, 128, 128), (65, 129, 65),
+          (128, 64, 31), (129, 200, 1000), (300, 257, 130), (257, 384, 4080)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("M,Nn,K", SHAPES)
+def test_linear_and_its_gradients(M, Nn, K, dtype):
+    g = torch.Generator(device=DEV).manual_seed(M + Nn + K)
+    w = weight(Nn, K, scale=0.3)
+    x = torch.randn(M, K, generator=g, device=DEV).to(dtype).requires_grad_()
+    b = torch.randn(Nn, generator=g, device=DEV).to(dtype).requires_grad_()
+    dy = torch.randn(M, Nn, generator=g, device=DEV).to(dtype)
+    y = mx4.linear(x, w, b)
+    dx, db = torch.autograd.grad(y, (x, b), dy)
+    w64, x64, d64 = w.dequantize().double(), x.detach().double(), dy.double()
+    ref = x64 @ w64.t() + b.detach().double()
+    assert y.dtype == dtype and float(((y.double() - ref).abs() - _bound(x64, w64, b.detach(), ref, K, PARTS[dtype], dtype)).max()) <= 0
+    rdx = d64 @ w64
+    assert dx.dtype == dtype and float(((dx.double() - rdx).abs() - _bound(d64, w64.t(), None, rdx, Nn, PARTS[dtype], dtype)).max()) <= 0
+    rdb = d64.sum(0)
+    tol = torch.finfo(dtype).eps / 2 * rdb.abs() + M * U * d64.abs().sum(0)
+    assert db.dtype == dtype and float(((db.double() - rdb).abs() - tol).max()) <= 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("M,Nn,K", SHAPES + [(1024, 512, 96), (500, 1030, 2050)])
+def test_product_of_two_4_bit_matrices(M, Nn, K, dtype):
+    a, w = weight(M, K, 1), weight(Nn, K, 2, 0.3)
+    b = torch.randn(Nn, device=DEV).to(dtype)
+    a64, w64 = a.dequantize().double(), w.dequantize().double()
+    for bias in (None, b):
+        y = mx4.linear(a, w, bias, out_dtype=dtype)
+        ref = a64 @ w64.t() + (0 if bias is None else bias.double())
+        assert y.dtype == dtype and float(((y.double() - ref).abs() - _bound(a64, w64, bias, ref, K, 1, dtype)).max()) <= 0
+
+
+@pytest.mark.parametrize("M", [1, 40, 200])
+def test_products_do_not_depend_on_what_lies_beside_them(M):
+    """Rows of a batch are the rows of the batch alone; repeated calls give the same bits."""
+    w = weight(96, 544, 3)
+    x = torch.randn(M, 544, device=DEV).to(BF16)
+    y = mx4.linear(x, w)
+    assert torch.equal(y, mx4.linear(x, w))
+    q = mx4.quantize(x)
+    p = mx4.linear(q, w, out_dtype=F32)
+    assert torch.equal(p, mx4.linear(q, w, out_dtype=F32))
+
+
+@pytest.mark.parametrize("M", [5, 100])
+def test_scales_over_the_whole_range(M):
+    # blocks whose scales differ by 2^200: products of large rows and small weights and the other way round
+    K, Nn = 96, 48
+    e = torch.tensor([-100.0, 0.0, 100.0], device=DEV).repeat_interleave(32)
+    wf = torch.randn(Nn, K, device=DEV) * torch.exp2(-e)
+    xf = torch.randn(M, K, device=DEV) * torch.exp2(e)
+    w = mx4.quantize(wf)
+    w64 = w.dequantize().double()
+    for x in (xf, xf.to(BF16)):
+        y, ref = mx4.linear(x, w), x.double() @ w64.t()
+        assert float(((y.double() - ref).abs() - _bound(x.double(), w64, None, ref, K, PARTS[x.dtype], x.dtype)).max()) <= 0
+    q = mx4.quantize(xf)
+    y, ref = mx4.linear(q, w), q.dequantize().double() @ w64.t()
+    assert float(((y.double() - ref).abs() - _bound(q.dequantize().double(), w64, None, ref, K, 1, F32)).max()) <= 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("M", [4, 100])
+def test_infinities_and_nan_stay_in_their_rows(M, dtype):
+    w = weight(70, 160, 4)
+    x = torch.randn(M, 160, device=DEV).to(dtype)
+    clean = mx4.linear(x, w)
+    x[1, 40] = float("inf")
+    x[3, 159] = float("nan")
+    y = mx4.linear(x, w)
+    keep = [i for i in range(M) if i not in (1, 3)]
+    assert torch.equal(y[keep], clean[keep]) and torch.isnan(y[3]).all()
+    col = w.dequantize()[:, 40]
+    want = torch.where(col == 0, torch.full_like(col, float("nan")), torch.sign(col) * float("inf"))   # inf * 0 is NaN
+    assert torch.equal(torch.isnan(y[1]), torch.isnan(want)) and torch.equal(y[1][col != 0].float(), want[col != 0])
+    # a NaN block of the weight or of the rows
+    s = w.scales.clone()
+    s[7, 2] = 255
+    z = mx4.linear(x[keep], mx4.MX4Tensor(w.codes, s, 160))
+    assert torch.isnan(z[:, 7]).all() and not torch.isnan(z[:, :7]).any() and not torch.isnan(z[:, 8:]).any()
+    q = mx4.linear(mx4.quantize(x), mx4.MX4Tensor(w.codes, s, 160))
+    assert torch.isnan(q[:, 7]).all() and torch.isnan(q[[1, 3]]).all()
+    rest = q[keep]
+    assert not torch.isnan(rest[:, :7]).any() and not torch.isnan(rest[:, 8:]).any()
+
+
+def test_largest_values_do_not_overflow_in_parts():
+    w = mx4.quantize(torch.full((16, 32), 2.0 ** -20, device=DEV))
+    x = torch.zeros(3, 32, device=DEV)
+    x[0, 3], x[1, 31], x[2, 0] = torch.finfo(F32).max, -torch.finfo(F32).max, 2.0 ** -140
+    ref = x.double() @ w.dequantize().double().t()
+    y = mx4.linear(x, w)
+    assert torch.isfinite(y).all() and float(((y.double() - ref).abs() - 100 * U * ref.abs()).max()) <= 2.0 ** -126
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("M", [3, 90])
+def test_strided_rows_and_leading_dimensions(M, dtype):
+    w = weight(50, 75, 5)
+    full = torch.randn(M, 91, device=DEV).to(dtype)
+    a = mx4.linear(full[:, 7:82], w)
+    assert torch.equal(a, mx4.linear(full[:, 7:82].contiguous(), w))
+    b = mx4.linear(full[:, 7:82].contiguous().view(M, 1, 75), w)
+    assert b.shape == (M, 1, 50) and torch.equal(b.view(M, 50), a)
+
+
+def test_rows_beyond_32_bit_offsets():
+    stride = 2 ** 30 + 8
+    buf = torch.empty(2 * stride + 200, dtype=BF16, device=DEV)
+    x = buf.as_strided((3, 200), (stride, 1))
+    vals = torch.randn(3, 200, device=DEV).to(BF16)
+    x.copy_(vals)
+    w = weight(40, 200, 6)
+    assert torch.equal(mx4.linear(x, w), mx4.linear(vals, w))
+    a, b = mx4.quantize(x), mx4.quantize(vals)
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+
+
+def test_empty_batches_and_absent_bias():
+    w = weight(24, 64, 7)
+    b = torch.ones(24, device=DEV, requires_grad=True)
+    x = torch.zeros(0, 64, device=DEV, requires_grad=True)
+    y = mx4.linear(x, w, b)
+    dx, db = torch.autograd.grad(y, (x, b), torch.zeros(0, 24, device=DEV))
+    assert y.shape == (0, 24) and dx.shape == (0, 64) and float(db.abs().max()) == 0
+    assert mx4.linear(mx4.quantize(x), w).shape == (0, 24)
+
+
+def test_many_rows_bias_gradient_in_fp32():
+    dy = torch.randn(70000, 40, device=DEV).to(BF16)
+    db = N.mx4_bias_grad(dy, F32)
+    ref = dy.double().sum(0)
+    assert float(((db.double() - ref).abs() - 70000 / 128 * U * dy.double().abs().sum(0)).max()) <= 0
+    assert torch.equal(db, N.mx4_bias_grad(dy, F32))
+
+
+def test_on_another_stream_and_in_a_recorded_graph():
+    w = weight(200, 320, 8)
+    x = torch.randn(90, 320, device=DEV).to(BF16).requires_grad_()
+    b = torch.randn(200, device=DEV).requires_grad_()
+    dy = torch.randn(90, 200, device=DEV).to(BF16)
+
+    def step(rows):
+        bias = b.detach().requires_grad_()      # a leaf of its own: no eager graph of it is alive when the step is recorded
+        y = mx4.linear(rows, w, bias)
+        grads = torch.autograd.grad(y, (rows, bias), dy)
+        q = mx4.linear(mx4.quantize(rows), w, b, out_dtype=F32)
+        few = mx4.linear(rows[:7].detach(), w, b)
+        return [y.detach(), *grads, q, few.detach()]
+
+    eager = step(x)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = step(x)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(p, q) for p, q in zip(eager, other))
+    xs = x.detach().clone().requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(xs)
+    for n in range(3):
+        with torch.no_grad():
+            xs.copy_(x.detach() * (n + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, step(xs.detach().clone().requires_grad_())))
+
+
+def test_layer_from_a_linear():
+    lin = torch.nn.Linear(96, 64).to(DEV)
+    layer = mx4.MX4Linear.from_linear(lin)
+    x = torch.randn(5, 3, 96, device=DEV)
+    q = mx4.quantize(lin.weight)
+    assert torch.equal(layer(x), mx4.linear(x, q, lin.bias))
+    state = layer.state_dict()
+    assert sorted(state) == ["bias", "codes", "scales"]
+    both = mx4.MX4Linear.from_linear(lin, activations="mx4")
+    with torch.no_grad():
+        assert torch.equal(both(x), mx4.linear(mx4.quantize(x), q, lin.bias).view(5, 3, 64))
+    with pytest.raises(N.NativeError, match="no_grad"):
+        both(x)
+
+
+def test_refusals_on_the_device():
+    w = weight(24, 64, 9)
+    x = torch.randn(3, 64, device=DEV)
+    with pytest.raises(N.NativeError, match="rows"):
+        mx4.linear(x[:, :60], w)
+    with pytest.raises(N.NativeError, match="results"):
+        mx4.linear(x, w, out_dtype=BF16)
+    with pytest.raises(N.NativeError, match="bias"):
+        mx4.linear(x, w, torch.ones(23, device=DEV))
+    with pytest.raises(N.NativeError, match="fp32, bf16 or fp16"):
+        mx4.linear(x.double(), w)
+    with pytest.raises(N.NativeError, match="not a 4-bit matrix"):
+        mx4.MX4Tensor(w.codes, w.scales, 65)
+    with pytest.raises(N.NativeError, match="aligned"):
+        mx4.MX4Tensor(torch.zeros(24 * 32 + 8, dtype=torch.uint8, device=DEV)[8:].view(24, 32), w.scales, 64)
+    with pytest.raises(N.NativeError, match="MX4Tensor"):
+        mx4.linear(x, x)
+    with pytest.raises(N.NativeError, match="is on cpu"):
+        mx4.linear(x, w, torch.ones(24))
+    with pytest.raises(N.NativeError):
+        mx4.quantize(torch.zeros(3, 4))
