@@ -79,6 +79,16 @@ __global__ __launch_bounds__(256) void k_mx4_dequantize(const uint8_t* __restric
     }
 }
 
+// Workgroup -> output tile.  Workgroups go round the eight XCDs, each with an L2 of its own: every XCD gets a run of consecutive
+// tiles in an order that walks columns of eight row tiles, so that the tiles in flight on it share rows and columns.
+__device__ __forceinline__ void mx4_tile_of(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
+    const int total = tiles_m * tiles_n, per = total / 8, extra = total % 8, xcd = id % 8;
+    const int pos = xcd * per + min(xcd, extra) + id / 8;
+    const int group = 8 * tiles_n, g = pos / group, first = g * 8, rows = min(8, tiles_m - first);
+    tm = first + (pos - g * group) % rows;
+    tn = (pos - g * group) / rows;
+}
+
 // ---- y = x W^T + bias, few rows -----------------------------------------------------------------------------------------
 // The weight is streamed once: a workgroup takes 16 weight rows, its waves split the blocks.  A lane holds one block of one
 // weight row (16 bytes, one scale) and feeds it to four matrix instructions, eight elements each; the four lane groups of an
@@ -222,52 +232,189 @@ __global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64
 }
 
 // ---- both operands in 4 bits ----------------------------------------------------------------------------------------------
-// One scaled matrix instruction takes a 16-byte block and its scale byte per lane from either operand: 16 x 16 outputs, 128 deep.
-template <typename T>
-__global__ __launch_bounds__(256) void k_mx4_product(Mx4 X, Mx4 W, const void* bias, int btype, T* __restrict__ y, int64_t ldy) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-    const int m0 = blockIdx.y * 64 + (w >> 1) * 32, n0 = blockIdx.x * 64 + (w & 1) * 32;
-    f32x4 acc[2][2];
+// Tiles of BM x BN outputs, 256 deep per step (eight blocks, 128 bytes a row), four waves, each owning WM x WN of 32x32x64 scaled
+// matrix instructions.  The codes go from memory to LDS as they are (16-byte direct loads, no registers in between), two buffers:
+// the loads of the next step run under the matrix instructions of this one.  A direct load fills LDS in lane order, so the lanes
+// choose their source instead: slot p of row r holds block p ^ (r & 7), and the 32 rows a fragment read touches fall on all banks.
+// An instruction's lane half h takes block 4 h + s of the step's eight in its s-th turn -- a permutation of the reduction index that
+// both operands share -- so that one dword holds a lane's four scales and the turn selects the byte.
+// Blocks behind the last one come from a zero block in memory, rows behind the last one repeat it and are not stored.
+__device__ const uint4 mx4_zero_block = {0u, 0u, 0u, 0u};
+
+struct __attribute__((packed, aligned(1))) Bytes8 { uint32_t lo, hi; };
+
+template <int BM, int BN>
+struct ProductStage {
+    __attribute__((aligned(16))) uint8_t x[BM * 128];
+    __attribute__((aligned(16))) uint8_t w[BN * 128];
+    uint32_t sx[BM * 2], sw[BN * 2];
+    uint32_t room[256];                  // (the 64 x 64 tile's output strips are a little longer than its codes)
+};
+
+template <int ROWS>
+__device__ __forceinline__ void mx4_stage_codes(const Mx4& A, int r0, int kb0, uint8_t* lds) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int lr = wave * 8 + (lane >> 3);
+    asm volatile("" : "+v"(lr));            // offsets are formed at each step: kept, they would take the accumulators' registers
+    const int c = (lane & 7) ^ (lane >> 3), last = A.rows - 1 - r0;
+    const uint8_t* base = A.codes + ((int64_t)r0 * A.nb + kb0) * 16;      // offsets inside a tile stay below 2^31 (checked at the call)
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int base = 0; base < W.nb; base += 4) {
-        const int kb = base + g;
-        const bool live = kb < W.nb;
-        i32x8 a[2], b[2];
-        int sa[2], sb[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int64_t n = (int64_t)min(n0 + i * 16 + c, W.rows - 1) * W.nb + kb, m = (int64_t)min(m0 + i * 16 + c, X.rows - 1) * X.nb + kb;
-            u32x4 qa{0, 0, 0, 0}, qb{0, 0, 0, 0};
-            sa[i] = sb[i] = 127;
-            if (live) {
-                qa = reinterpret_cast<const u32x4*>(W.codes)[n];
-                qb = reinterpret_cast<const u32x4*>(X.codes)[m];
-                sa[i] = W.scales[n];
-                sb[i] = X.scales[m];
-            }
-            a[i] = i32x8{(int)qa[0], (int)qa[1], (int)qa[2], (int)qa[3], 0, 0, 0, 0};
-            b[i] = i32x8{(int)qb[0], (int)qb[1], (int)qb[2], (int)qb[3], 0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b[j], acc[i][j], 4, 4, 0, sa[i], 0, sb[j]);
+    for (int j = 0; j < ROWS / 32; ++j) {
+        const uint8_t* src = base + (uint32_t)((min(lr + j * 32, last) * A.nb + c) * 16);
+        src = kb0 + c < A.nb ? src : reinterpret_cast<const uint8_t*>(&mx4_zero_block);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src,
+                                         (__attribute__((address_space(3))) uint32_t*)(lds + (j * 4 + wave) * 1024), 16, 0, 0);
     }
+}
+// the scale bytes of a row's blocks [kb0, kb0 + 8), 0 behind the last one; nb >= 8 (no branch: the row's last eight, shifted when
+// they are put away, so that nothing waits for the load before)
+__device__ __forceinline__ Bytes8 mx4_row_scales(const Mx4& A, int row, int kb0) {
+    return *reinterpret_cast<const Bytes8*>(A.scales + (int64_t)min(row, A.rows - 1) * A.nb + min(kb0, A.nb - 8));
+}
+__device__ __forceinline__ uint2 mx4_shift_scales(Bytes8 b, int nb, int kb0) {
+    const int shift = min(kb0 - min(kb0, nb - 8), 7) * 8;
+    const uint64_t v = ((uint64_t)b.hi << 32 | b.lo) >> shift;
+    return make_uint2((uint32_t)v, (uint32_t)(v >> 32));
+}
+// the same for a row of fewer than eight blocks
+__device__ __forceinline__ uint2 mx4_short_row_scales(const Mx4& A, int row) {
+    const uint8_t* p = A.scales + (int64_t)min(row, A.rows - 1) * A.nb;
+    uint64_t v = 0;
+    for (int i = 0; i < A.nb; ++i) v |= (uint64_t)p[i] << (8 * i);
+    return make_uint2((uint32_t)v, (uint32_t)(v >> 32));
+}
+
+// fragments of turn S of a step, and the matrix instructions of a turn
+template <int S, int TM, int TN>
+__device__ __forceinline__ void mx4_turn_load(const uint8_t* x, const uint8_t* w, u32x4 (&b)[TM], u32x4 (&a)[TN]) {
+    const int lane = threadIdx.x & 63;
+    const int at = (lane & 31) * 128 + ((((lane >> 5) * 4 + S) ^ (lane & 7)) * 16);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < TN; ++i) a[i] = *reinterpret_cast<const u32x4*>(w + i * 32 * 128 + at);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int m = m0 + j * 16 + c;
+    for (int j = 0; j < TM; ++j) b[j] = *reinterpret_cast<const u32x4*>(x + j * 32 * 128 + at);
+}
+__device__ __forceinline__ i32x8 mx4_operand(const u32x4& q) { return i32x8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0}; }
+template <int S, int TM, int TN>
+__device__ __forceinline__ void mx4_turn(const u32x4 (&b)[TM], const u32x4 (&a)[TN], const int (&sx)[TM], const int (&sw)[TN], f32x16 (&acc)[TN][TM]) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int n = n0 + i * 16 + 4 * g + e;
-                if (m < X.rows && n < W.rows) y[m * ldy + n] = (T)(acc[i][j][e] + (bias != nullptr ? load_elem(bias, btype, n) : 0.f));
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx4_operand(a[i]), mx4_operand(b[j]), acc[i][j], 4, 4, S, sw[i], S, sx[j]);
+}
+
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(256) void k_mx4_product(Mx4 X, Mx4 W, const void* bias, int btype, T* __restrict__ y, int64_t ldy, int tiles_m,
+                                                     int tiles_n) {
+    static_assert((BM / WM) * (BN / WN) == 4, "four waves");
+    constexpr int TM = WM / 32, TN = WN / 32;
+    using Stage = ProductStage<BM, BN>;
+    constexpr int OUT_LD = WN + 4;                                // floats per row of the output strip
+    static_assert(sizeof(Stage) >= 4 * 32 * OUT_LD * sizeof(float), "the output strips fit one stage");
+    __shared__ Stage s0, s1;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int tm, tn;
+    mx4_tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    const int m0 = tm * BM, n0 = tn * BN, wm = (wave / (BN / WN)) * WM, wn = (wave % (BN / WN)) * WN;
+    f32x16 acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    // scales: thread t brings row t of the x tile and row t of the w tile
+    auto scales = [&](int kb0, Bytes8& vx, Bytes8& vw) {
+        vx = mx4_row_scales(X, m0 + (threadIdx.x & (BM - 1)), kb0);
+        vw = mx4_row_scales(W, n0 + (threadIdx.x & (BN - 1)), kb0);
+    };
+    auto put = [&](Stage& st, uint2 vx, uint2 vw) {
+        *reinterpret_cast<uint2*>(&st.sx[(threadIdx.x & (BM - 1)) * 2]) = vx;      // (smaller tiles: the same value more than once)
+        *reinterpret_cast<uint2*>(&st.sw[(threadIdx.x & (BN - 1)) * 2]) = vw;
+    };
+    auto put_scales = [&](Stage& st, int kb0, Bytes8 vx, Bytes8 vw) { put(st, mx4_shift_scales(vx, W.nb, kb0), mx4_shift_scales(vw, W.nb, kb0)); };
+    auto codes = [&](Stage& st, int kb0) {
+        mx4_stage_codes<BM>(X, m0, kb0, st.x);
+        mx4_stage_codes<BN>(W, n0, kb0, st.w);
+    };
+    auto compute = [&](const Stage& st) {
+        int sx[TM], sw[TN];
+#pragma unroll
+        for (int j = 0; j < TM; ++j) sx[j] = (int)st.sx[(wm + j * 32 + (lane & 31)) * 2 + (lane >> 5)];
+#pragma unroll
+        for (int i = 0; i < TN; ++i) sw[i] = (int)st.sw[(wn + i * 32 + (lane & 31)) * 2 + (lane >> 5)];
+        // the next turn's fragments are on their way while this turn's instructions run
+        const uint8_t *x = st.x + wm * 128, *w = st.w + wn * 128;
+        u32x4 b0[TM], a0[TN], b1[TM], a1[TN];
+        mx4_turn_load<0, TM, TN>(x, w, b0, a0);
+        mx4_turn_load<1, TM, TN>(x, w, b1, a1);
+        mx4_turn<0, TM, TN>(b0, a0, sx, sw, acc);
+        __builtin_amdgcn_sched_barrier(0);
+        mx4_turn_load<2, TM, TN>(x, w, b0, a0);
+        mx4_turn<1, TM, TN>(b1, a1, sx, sw, acc);
+        __builtin_amdgcn_sched_barrier(0);
+        mx4_turn_load<3, TM, TN>(x, w, b1, a1);
+        mx4_turn<2, TM, TN>(b0, a0, sx, sw, acc);
+        __builtin_amdgcn_sched_barrier(0);
+        mx4_turn<3, TM, TN>(b1, a1, sx, sw, acc);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    Bytes8 vx{0u, 0u}, vw{0u, 0u};
+    codes(s0, 0);
+    if (W.nb >= 8) {
+        scales(0, vx, vw);
+        put_scales(s0, 0, vx, vw);
+    } else {
+        put(s0, mx4_short_row_scales(X, m0 + (threadIdx.x & (BM - 1))), mx4_short_row_scales(W, n0 + (threadIdx.x & (BN - 1))));
+    }
+    __syncthreads();
+    const int steps = (W.nb + 7) / 8;
+    for (int p = 0; p < steps / 2; ++p) {
+        const int kb1 = p * 16 + 8, kb2 = kb1 + 8;
+        scales(kb1, vx, vw);
+        codes(s1, kb1);
+        compute(s0);
+        put_scales(s1, kb1, vx, vw);
+        __syncthreads();
+        scales(kb2, vx, vw);
+        codes(s0, kb2);                     // behind the last step: zero blocks, not used
+        compute(s1);
+        put_scales(s0, kb2, vx, vw);
+        __syncthreads();
+    }
+    if (steps & 1) compute(s0);
+    __syncthreads();
+    // outputs: a wave turns 32 rows at a time through LDS so that rows leave in 16-byte pieces
+    constexpr int VEC = Elem<T>::VEC, LPR = WN / VEC;             // lanes per row
+    float* strip = reinterpret_cast<float*>(&s0) + wave * 32 * OUT_LD;
+    float bv[VEC];
+    const int nl = (lane % LPR) * VEC, n = n0 + wn + nl;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) bv[i] = bias != nullptr && n + i < W.rows ? load_elem(bias, btype, n + i) : 0.f;
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<f32x4*>(&strip[(lane & 31) * OUT_LD + i * 32 + 8 * q + 4 * (lane >> 5)]) =
+                    f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        // only this wave uses the strip: its own LDS accesses stay in order
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < 32; r += 64 / LPR) {
+            const int row = r + lane / LPR, m = m0 + wm + j * 32 + row;
+            float v[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; i += 4) {
+                const f32x4 f = *reinterpret_cast<const f32x4*>(&strip[row * OUT_LD + nl + i]);
+                v[i] = f[0] + bv[i]; v[i + 1] = f[1] + bv[i + 1]; v[i + 2] = f[2] + bv[i + 2]; v[i + 3] = f[3] + bv[i + 3];
             }
+            if (m < X.rows && n < W.rows) store_slot(y + m * ldy, n, W.rows, v);
         }
+        __builtin_amdgcn_wave_barrier();
+    }
 }
 
 // ---- bias gradient: column sums of dy ----------------------------------------------------------------------------------
@@ -413,13 +560,25 @@ extern "C" int drm_mx4_product(const uint8_t* x_codes, const uint8_t* x_scales, 
     if (int rc = mx4_check(__func__, x_codes, x_scales, M, K)) return rc;
     if (int rc = mx4_check(__func__, w_codes, w_scales, N, K)) return rc;
     if (int rc = mx4_check_product(__func__, x_codes, K, y_dtype, K, bias, bias_dtype, y, ldy, N, M)) return rc;
-    if (int rc = mx4_check_grid(__func__, M, 64)) return rc;
+    DRM_REQUIRE(K <= (1 << 22), DRM_ENOTSUP, "K=%d (at most 4194304)", K);
+    DRM_REQUIRE((int64_t)((M + 63) / 64) * ((N + 63) / 64) <= INT_MAX, DRM_ENOTSUP, "M=%d N=%d: too many tiles", M, N);
     hipStream_t s = (hipStream_t)stream;
     const Mx4 X{x_codes, x_scales, M, mx4_blocks(K)}, W{w_codes, w_scales, N, mx4_blocks(K)};
     ProfScope ps(PC_LINEAR_BIG, s, 2.0 * M * N * K, (double)M * N * elem_bytes(y_dtype) + ((double)M + N) * W.nb * 17);
     return with_elem(y_dtype, [&](auto tag) -> int {
         using T = decltype(tag);
-        k_mx4_product<T><<<dim3((N + 63) / 64, (M + 63) / 64), 256, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy);
+        // the largest tile (fewest bytes through LDS per product) whose tiles still give every CU one
+        auto tiles = [&](int b) { return (int64_t)((M + b - 1) / b) * ((N + b - 1) / b); };
+        if (tiles(256) >= 192) {
+            const int tm = (M + 255) / 256, tn = (N + 255) / 256;
+            k_mx4_product<T, 256, 256, 128, 128><<<tm * tn, 256, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy, tm, tn);
+        } else if (tiles(128) >= 192) {
+            const int tm = (M + 127) / 128, tn = (N + 127) / 128;
+            k_mx4_product<T, 128, 128, 64, 64><<<tm * tn, 256, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy, tm, tn);
+        } else {
+            const int tm = (M + 63) / 64, tn = (N + 63) / 64;
+            k_mx4_product<T, 64, 64, 32, 32><<<tm * tn, 256, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy, tm, tn);
+        }
         DRM_LAUNCH_CHECK();
         return DRM_OK;
     });

@@ -148,7 +148,7 @@ def test_linear_and_its_gradients(M, Nn, K, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("M,Nn,K", SHAPES + [(1024, 512, 96), (500, 1030, 2050)])
+@pytest.mark.parametrize("M,Nn,K", SHAPES + [(1024, 512, 96), (500, 1030, 2050), (1700, 1750, 200), (3900, 3601, 130), (4000, 3500, 1290)])
 def test_product_of_two_4_bit_matrices(M, Nn, K, dtype):
     a, w = weight(M, K, 1), weight(Nn, K, 2, 0.3)
     b = torch.randn(Nn, device=DEV).to(dtype)
