@@ -141,18 +141,99 @@ __global__ __launch_bounds__(NW * 64) void k_mx4_rows(const T* __restrict__ x, i
     }
 }
 
+// what lies behind the last block of a row: sixteen zero bytes in memory
+__device__ const uint4 mx4_zero_block = {0u, 0u, 0u, 0u};
+
+// A row's NB blocks of a step in LDS: block b in slot b ^ (the row's number), so that eight rows of one block fall on all banks
+template <int NB>
+__device__ __forceinline__ int mx4_code_slot(int r, int b) { return NB == 4 ? b ^ ((r >> 1) & 3) : b ^ ((r >> 2) & 1); }
+
+// Outputs of a wave (WM rows x WN columns in 32x32 accumulators whose lanes are rows): 32 rows at a time turn through LDS, so that
+// they leave in 16-byte pieces of a row.  `strip`: 32 x (WN + 4) floats of this wave's own.
+template <typename T, int WM, int WN>
+__device__ __forceinline__ void mx4_store_tile(float* strip, const f32x16 (&acc)[WN / 32][WM / 32], T* __restrict__ y, int64_t ldy, int m0,
+                                               int n0, int M, int N, const void* bias, int btype) {
+    constexpr int LD = WN + 4, VEC = Elem<T>::VEC, LPR = WN / VEC;             // lanes per row
+    const int lane = threadIdx.x & 63, nl = (lane % LPR) * VEC, n = n0 + nl;
+    float bv[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) bv[i] = bias != nullptr && n + i < N ? load_elem(bias, btype, n + i) : 0.f;
+#pragma unroll
+    for (int j = 0; j < WM / 32; ++j) {
+#pragma unroll
+        for (int i = 0; i < WN / 32; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<f32x4*>(&strip[(lane & 31) * LD + i * 32 + 8 * q + 4 * (lane >> 5)]) =
+                    f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        __builtin_amdgcn_wave_barrier();        // one wave's LDS accesses stay in order
+#pragma unroll
+        for (int r = 0; r < 32; r += 64 / LPR) {
+            const int row = r + lane / LPR, m = m0 + j * 32 + row;
+            float v[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; i += 4) {
+                const f32x4 f = *reinterpret_cast<const f32x4*>(&strip[row * LD + nl + i]);
+                v[i] = f[0] + bv[i]; v[i + 1] = f[1] + bv[i + 1]; v[i + 2] = f[2] + bv[i + 2]; v[i + 3] = f[3] + bv[i + 3];
+            }
+            if (m < M && n < N) store_slot(y + m * ldy, n, N, v);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
 // ---- y = x W^T + bias and dx = dy W, many rows --------------------------------------------------------------------------
-// 128 x 128 output tile, reduction in steps of 64; the 4-bit operand is widened to bf16 on its way into LDS (for dx: transposed),
-// the float operand goes there in its bf16 parts.  LDS rows of 64 elements = 8 chunks of 16 bytes, chunk c of row r at c ^ (r & 7).
-template <typename T, bool GRAD>
+// 128 x 128 outputs per workgroup, four waves of 64 x 64 (32x32x16 bf16 matrix instructions), BK of the reduction per step, two
+// LDS stages.  The float operand lies in LDS in its bf16 parts: rows of BK, 16-byte chunk c of row r at c ^ (r & 7); bf16 rows
+// whose chunks are aligned go there by direct loads, others through registers.
+//   y : the codes lie in LDS as they are and every wave widens the fragments it needs (an eighth of the LDS traffic of
+//       bf16 rows; the conversion instruction takes a quarter of the vector rate, half of the matrix instructions' time).
+//   dx: the reduction runs over W's rows, so that a fragment needs one column of eight rows: the block of a row is widened
+//       once, four rows side by side exchange their dwords (a transposition among four lanes), and the columns go to LDS.
+template <typename T, int BK, bool DIRECT, bool GRAD>
+struct TileStage {
+    static constexpr int P = Parts<T>::N, NB = BK / 32;
+    __attribute__((aligned(16))) uint8_t x[P][128 * BK * 2];
+    __attribute__((aligned(16))) uint8_t w[GRAD ? 128 * BK * 2 : 128 * NB * 16];
+    uint32_t sw[GRAD ? 4 : 128];
+};
+
+// position of chunk c in row r of a tile of bf16 rows
+__device__ __forceinline__ int mx4_chunk(int r, int c) { return (c & 8) | ((c ^ r) & 7); }
+// dx: columns of W; eight of them are written by lanes of one instruction, so their number takes part as well
+__device__ __forceinline__ int mx4_chunk_t(int r, int c) { return (c & 8) | ((c ^ r ^ (r >> 3)) & 7); }
+
+struct __attribute__((packed, aligned(1))) Bytes4 { uint32_t v; };
+struct __attribute__((packed, aligned(1))) Bytes2 { uint16_t v; };
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t quad(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false); }
+
+// One block (16 bytes) of each of four rows that sit in the four lanes of a quad -> lane q: codes 8 q .. 8 q + 7 of the four rows
+__device__ __forceinline__ u32x4 quad_transpose(u32x4 d, int q) {
+    const bool odd = q & 1, high = q & 2;
+    uint32_t t0 = quad<0xB1>(odd ? d[0] : d[1]), t1 = quad<0xB1>(odd ? d[2] : d[3]);
+    if (odd) { d[0] = t0; d[2] = t1; } else { d[1] = t0; d[3] = t1; }
+    t0 = quad<0x4E>(high ? d[0] : d[2]);
+    t1 = quad<0x4E>(high ? d[1] : d[3]);
+    if (high) { d[0] = t0; d[1] = t1; } else { d[2] = t0; d[3] = t1; }
+    return d;
+}
+
+template <typename T, int BK, bool DIRECT, bool GRAD>
 __global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64_t ldx, Mx4 W, const void* bias, int btype,
-                                                  T* __restrict__ y, int64_t ldy, int M, int N, int K) {
-    // forward: reduction over W's columns (K), output columns are W's rows; gradient: the other way round (N = output columns)
-    constexpr int P = Parts<T>::N, BK = 64;
-    __shared__ __attribute__((aligned(16))) uint16_t s_x[P][128 * BK];
-    __shared__ __attribute__((aligned(16))) uint16_t s_w[128 * BK];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int m0 = blockIdx.y * 128, n0 = blockIdx.x * 128, wm = (w >> 1) * 64, wn = (w & 1) * 64;
+                                                  T* __restrict__ y, int64_t ldy, int M, int N, int K, int tiles_m, int tiles_n) {
+    // y: reduction over W's columns (K of them), N = W's rows; dx: reduction over W's rows (K of them), N = W's columns
+    static_assert(!DIRECT || Parts<T>::N == 1, "direct loads bring bf16");
+    using Stage = TileStage<T, BK, DIRECT, GRAD>;
+    constexpr int P = Stage::P, NB = Stage::NB, CH = BK / 8, XU = 128 * CH / 256, WU = GRAD ? BK / 64 : 1;
+    constexpr int OUT_LD = 64 + 4;
+    static_assert(sizeof(Stage) >= 4 * 32 * OUT_LD * sizeof(float), "the output strips fit one stage");
+    __shared__ Stage s0, s1;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
+    int tm, tn;
+    mx4_tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    const int m0 = tm * 128, n0 = tn * 128, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
     f32x16 acc[2][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -160,75 +241,206 @@ __global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    for (int k0 = 0; k0 < K; k0 += BK) {
-        __syncthreads();
-        for (int o = threadIdx.x; o < 128 * 8; o += 256) {
-            const int r = o >> 3, ch = o & 7;
-            bf16x8 p[P];
-            load_parts(x + (int64_t)min(m0 + r, M - 1) * ldx, k0 + ch * 8, K, p);
+
+    struct Held {                     // what a step brings through registers
+        Eight<T> x[DIRECT ? 1 : XU];
+        u32x4 w[WU];
+        uint32_t sw[WU];
+    };
+    auto load_scales = [&](int k0, Held& h) {       // W.nb >= NB: the row's bytes of this step, or its last ones, shifted by put
+        const uint8_t* p = W.scales + (int64_t)min(n0 + (int)(threadIdx.x & 127), N - 1) * W.nb + min(k0 >> 5, W.nb - NB);
+        if constexpr (NB == 4) h.sw[0] = reinterpret_cast<const Bytes4*>(p)->v;
+        else h.sw[0] = reinterpret_cast<const Bytes2*>(p)->v;
+    };
+    const int whole = DIRECT ? K : K & ~7;        // elements of a row in whole chunks (direct loads: all of them)
+    auto load = [&](Stage& st, int k0, Held& h, bool tail) {
+        if constexpr (GRAD) {
 #pragma unroll
-            for (int q = 0; q < P; ++q) *reinterpret_cast<bf16x8*>(&s_x[q][r * BK + ((ch ^ (r & 7)) * 8)]) = p[q];
+            for (int j = 0; j < WU; ++j) {
+                const int u = threadIdx.x + 256 * j, n = k0 + (u >> 4) * 4 + (u & 3), kb = (n0 >> 5) + ((u >> 2) & 3);
+                const int64_t at = (int64_t)min(n, W.rows - 1) * W.nb + min(kb, W.nb - 1);
+                h.sw[j] = W.scales[at];
+                h.w[j] = reinterpret_cast<const u32x4*>(W.codes)[at];
+            }
         }
-        if constexpr (!GRAD) {
-            for (int o = threadIdx.x; o < 128 * 8; o += 256) {
-                const int r = o >> 3, ch = o & 7, kb = (k0 >> 5) + (ch >> 2);
-                const int64_t n = min(n0 + r, N - 1);
-                bf16x8 v = mx4_bf16x8(0u, 1.f);
-                if (kb < W.nb)
-                    v = mx4_bf16x8(reinterpret_cast<const uint32_t*>(W.codes)[(n * W.nb + kb) * 4 + (ch & 3)], mx4_scale(W.scales[n * W.nb + kb]));
-                *reinterpret_cast<bf16x8*>(&s_w[r * BK + ((ch ^ (r & 7)) * 8)]) = v;
+        if constexpr (DIRECT) {
+            constexpr int RPI = 64 / CH;                          // rows per wave and instruction
+            const int row = lane / CH;
+            const int c = mx4_chunk(row, lane % CH);              // (an involution; rows advance by multiples of RPI)
+            const uint8_t* base = reinterpret_cast<const uint8_t*>(x + (int64_t)m0 * ldx + k0);
+#pragma unroll
+            for (int j = 0; j < 128 / RPI / 4; ++j) {
+                const int r = (j * 4 + wave) * RPI + row;
+                const int cc = RPI == 8 ? c : mx4_chunk(r, lane % CH);
+                const uint8_t* src = base + (uint32_t)(min(r, M - 1 - m0) * (int)ldx * 2 + cc * 16);
+                src = k0 + cc * 8 < K ? src : reinterpret_cast<const uint8_t*>(&mx4_zero_block);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src,
+                                                 (__attribute__((address_space(3))) uint32_t*)(st.x[0] + (j * 4 + wave) * 1024), 16, 0, 0);
             }
         } else {
-            // eight codes of one weight row (columns n0 + ...) per step, scattered down a column of the tile
-            for (int o = threadIdx.x; o < 64 * 16; o += 256) {
-                const int rr = o >> 4, c8 = o & 15, col = n0 + c8 * 8, kb = col >> 5;
-                const int64_t n = k0 + rr;
-                bf16x8 v = mx4_bf16x8(0u, 1.f);
-                if (n < W.rows && kb < W.nb)
-                    v = mx4_bf16x8(reinterpret_cast<const uint32_t*>(W.codes)[(n * W.nb + kb) * 4 + ((col >> 3) & 3)], mx4_scale(W.scales[n * W.nb + kb]));
+            // whole chunks of eight; what is left of a row behind them follows in a step of its own
+            if (!tail) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int r = c8 * 8 + i;
-                    s_w[r * BK + (((rr >> 3) ^ (r & 7)) * 8) + (rr & 7)] = __builtin_bit_cast(uint16_t, (__bf16)v[i]);
+                for (int j = 0; j < XU; ++j) {
+                    const int u = threadIdx.x + 256 * j, r = u / CH, c = u % CH;
+                    h.x[j] = reinterpret_cast<const Packed8<T>*>(x + (int64_t)min(m0 + r, M - 1) * ldx + max(min(k0 + c * 8, whole - 8), 0))->e;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < XU; ++j) {
+                    const int u = threadIdx.x + 256 * j, r = u / CH, c = u % CH;
+                    h.x[j] = load_eight(x + (int64_t)min(m0 + r, M - 1) * ldx, k0 + c * 8 < whole ? (int64_t)K : (int64_t)k0 + c * 8, K);
                 }
             }
         }
-        __syncthreads();
+        if constexpr (!GRAD) {
+            const uint8_t* base = W.codes + ((int64_t)n0 * W.nb + (k0 >> 5)) * 16;
 #pragma unroll
-        for (int s = 0; s < BK / 16; ++s) {
-            bf16x8 a[2], b[2];
-            const int ch = s * 2 + (lane >> 5);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = wn + i * 32 + (lane & 31);
-                a[i] = *reinterpret_cast<const bf16x8*>(&s_w[r * BK + ((ch ^ (r & 7)) * 8)]);
+            for (int j = 0; j < NB / 2; ++j) {
+                const int r = (j * 4 + wave) * (64 / NB) + lane / NB, b = mx4_code_slot<NB>(r, lane % NB);
+                const uint8_t* src = base + (uint32_t)((min(r, N - 1 - n0) * W.nb + b) * 16);
+                src = (k0 >> 5) + b < W.nb ? src : reinterpret_cast<const uint8_t*>(&mx4_zero_block);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src,
+                                                 (__attribute__((address_space(3))) uint32_t*)(st.w + (j * 4 + wave) * 1024), 16, 0, 0);
             }
+        }
+    };
+    auto put = [&](Stage& st, int k0, const Held& h, bool tail) {
+        if constexpr (!DIRECT) {
 #pragma unroll
-            for (int p = P - 1; p >= 0; --p) {
+            for (int j = 0; j < XU; ++j) {
+                const int u = threadIdx.x + 256 * j, r = u / CH, c = u % CH;
+                bf16x8 p[P];
+                split_eight<T>(tail || k0 + c * 8 < whole ? h.x[j] : Eight<T>{}, p);
+#pragma unroll
+                for (int q = 0; q < P; ++q) *reinterpret_cast<bf16x8*>(st.x[q] + r * BK * 2 + mx4_chunk(r, c) * 16) = p[q];
+            }
+        }
+        if constexpr (!GRAD) {
+            const int kb0 = k0 >> 5;
+            st.sw[threadIdx.x & 127] = h.sw[0] >> (min(kb0 - min(kb0, max(W.nb - NB, 0)), NB - 1) * 8);
+        } else {
+#pragma unroll
+            for (int j = 0; j < WU; ++j) {
+                const int u = threadIdx.x + 256 * j, q = u & 3;
+                const bool live = k0 + (u >> 4) * 4 + q < W.rows && (n0 >> 5) + ((u >> 2) & 3) < W.nb;
+                const u32x4 d = quad_transpose(live ? h.w[j] : u32x4{0u, 0u, 0u, 0u}, q);
+                const uint32_t own = live ? h.sw[j] : 127u;
+                const float sc[4] = {mx4_scale(quad<0x00>(own)), mx4_scale(quad<0x55>(own)), mx4_scale(quad<0xAA>(own)), mx4_scale(quad<0xFF>(own))};
+                u32x4 r[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(u32x4, mx4_bf16x8(d[i], sc[i]));
+                const int col = ((u >> 2) & 3) * 32 + q * 8, at = (u >> 4) * 4;     // eight columns, four rows of W
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint2 lo = make_uint2(__builtin_amdgcn_perm(r[1][i], r[0][i], 0x05040100u), __builtin_amdgcn_perm(r[3][i], r[2][i], 0x05040100u));
+                    const uint2 hi = make_uint2(__builtin_amdgcn_perm(r[1][i], r[0][i], 0x07060302u), __builtin_amdgcn_perm(r[3][i], r[2][i], 0x07060302u));
+                    const int c0 = col + 2 * i, c1 = c0 + 1;
+                    *reinterpret_cast<uint2*>(st.w + c0 * BK * 2 + mx4_chunk_t(c0, at >> 3) * 16 + (at & 4) * 2) = lo;
+                    *reinterpret_cast<uint2*>(st.w + c1 * BK * 2 + mx4_chunk_t(c1, at >> 3) * 16 + (at & 4) * 2) = hi;
+                }
+            }
+        }
+    };
+    // A turn (16 of the reduction) fetches the next turn's fragments beside its own matrix instructions: x from LDS, the widened
+    // codes of a block that was read a turn earlier.  (y: a lane half holds 16 codes in a row, eight per turn; dx: in order.)
+    struct Turn { bf16x8 a[2], v[P][2]; };
+    auto compute = [&](const Stage& st) {
+        uint32_t sw[2] = {0u, 0u};
+        uint2 q[2][2];
+        Turn f[2];
+        if constexpr (!GRAD) { sw[0] = st.sw[wn + l32]; sw[1] = st.sw[wn + 32 + l32]; }
+        auto codes = [&](int b) {
+            if constexpr (!GRAD) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = wn + i * 32 + l32;
+                    q[b & 1][i] = *reinterpret_cast<const uint2*>(st.w + r * NB * 16 + mx4_code_slot<NB>(r, b) * 16 + half * 8);
+                }
+            }
+        };
+        auto fetch = [&](int t) {
+            const int b = t >> 1, c = GRAD ? t * 2 + half : b * 4 + half * 2 + (t & 1);
+#pragma unroll
+            for (int p = 0; p < P; ++p)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const int r = wm + j * 32 + (lane & 31);
-                    b[j] = *reinterpret_cast<const bf16x8*>(&s_x[p][r * BK + ((ch ^ (r & 7)) * 8)]);
+                    const int r = wm + j * 32 + l32;
+                    f[t & 1].v[p][j] = *reinterpret_cast<const bf16x8*>(st.x[p] + r * BK * 2 + mx4_chunk(r, c) * 16);
                 }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if constexpr (GRAD) {
+                    const int r = wn + i * 32 + l32;
+                    f[t & 1].a[i] = *reinterpret_cast<const bf16x8*>(st.w + r * BK * 2 + mx4_chunk_t(r, c) * 16);
+                } else {
+                    f[t & 1].a[i] = mx4_bf16x8((t & 1) == 0 ? q[b & 1][i].x : q[b & 1][i].y, mx4_scale((sw[i] >> (8 * b)) & 255u));
+                }
+            }
+        };
+        codes(0);
+        fetch(0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < 2 * NB; ++t) {
+            if ((t & 1) == 0 && t / 2 + 1 < NB) codes(t / 2 + 1);
+            if (t + 1 < 2 * NB) fetch(t + 1);
+#pragma unroll
+            for (int p = P - 1; p >= 0; --p)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < 2; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[t & 1].a[i], f[t & 1].v[p][j], acc[i][j], 0, 0, 0);
+#pragma unroll
+            for (int k = 0; k < 4 * P; ++k) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
             }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    Held h;
+    if constexpr (!GRAD) {
+        if (W.nb >= NB) {
+            load_scales(0, h);
+        } else {                          // a row shorter than a step (then there is no second one)
+            h.sw[0] = 0u;
+            for (int i = 0; i < W.nb; ++i)
+                h.sw[0] |= (uint32_t)W.scales[(int64_t)min(n0 + (int)(threadIdx.x & 127), N - 1) * W.nb + i] << (8 * i);
         }
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int m = m0 + wm + j * 32 + (lane & 31);
-            if (m >= M) continue;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int n = n0 + wn + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-                if (n < N) y[m * ldy + n] = (T)(acc[i][j][e] + (bias != nullptr ? load_elem(bias, btype, n) : 0.f));
-            }
+    const int steps = (whole + BK - 1) / BK;
+    if (steps > 0) {
+        load(s0, 0, h, false);
+        put(s0, 0, h, false);
+        __syncthreads();
+        for (int p = 0; p < steps / 2; ++p) {
+            const int k1 = (2 * p + 1) * BK, k2 = k1 + BK;
+            if constexpr (!GRAD) load_scales(k1, h);      // first: nothing behind it has to wait for the rest
+            load(s1, k1, h, false);
+            compute(s0);
+            put(s1, k1, h, false);
+            __syncthreads();
+            if constexpr (!GRAD) load_scales(k2, h);
+            load(s0, k2, h, false);                       // behind the last step: not used
+            compute(s1);
+            put(s0, k2, h, false);
+            __syncthreads();
         }
+        if (steps & 1) compute(s0);
+    }
+    if (!DIRECT && whole < K) {
+        const int k0 = whole / BK * BK;
+        if constexpr (!GRAD) { if (k0 > 0) load_scales(k0, h); }
+        load(s1, k0, h, true);
+        put(s1, k0, h, true);
+        __syncthreads();
+        compute(s1);
+    }
+    __syncthreads();
+    mx4_store_tile<T, 64, 64>(reinterpret_cast<float*>(&s0) + wave * 32 * OUT_LD, acc, y, ldy, m0 + wm, n0 + wn, M, N, bias, btype);
 }
 
 // ---- both operands in 4 bits ----------------------------------------------------------------------------------------------
@@ -238,9 +450,7 @@ __global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64
 // choose their source instead: slot p of row r holds block p ^ (r & 7), and the 32 rows a fragment read touches fall on all banks.
 // An instruction's lane half h takes block 4 h + s of the step's eight in its s-th turn -- a permutation of the reduction index that
 // both operands share -- so that one dword holds a lane's four scales and the turn selects the byte.
-// Blocks behind the last one come from a zero block in memory, rows behind the last one repeat it and are not stored.
-__device__ const uint4 mx4_zero_block = {0u, 0u, 0u, 0u};
-
+// Blocks behind the last one come from the zero block, rows behind the last one repeat it and are not stored.
 struct __attribute__((packed, aligned(1))) Bytes8 { uint32_t lo, hi; };
 
 template <int BM, int BN>
@@ -385,36 +595,7 @@ __global__ __launch_bounds__(256) void k_mx4_product(Mx4 X, Mx4 W, const void* b
     }
     if (steps & 1) compute(s0);
     __syncthreads();
-    // outputs: a wave turns 32 rows at a time through LDS so that rows leave in 16-byte pieces
-    constexpr int VEC = Elem<T>::VEC, LPR = WN / VEC;             // lanes per row
-    float* strip = reinterpret_cast<float*>(&s0) + wave * 32 * OUT_LD;
-    float bv[VEC];
-    const int nl = (lane % LPR) * VEC, n = n0 + wn + nl;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) bv[i] = bias != nullptr && n + i < W.rows ? load_elem(bias, btype, n + i) : 0.f;
-#pragma unroll
-    for (int j = 0; j < TM; ++j) {
-#pragma unroll
-        for (int i = 0; i < TN; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                *reinterpret_cast<f32x4*>(&strip[(lane & 31) * OUT_LD + i * 32 + 8 * q + 4 * (lane >> 5)]) =
-                    f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-        // only this wave uses the strip: its own LDS accesses stay in order
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int r = 0; r < 32; r += 64 / LPR) {
-            const int row = r + lane / LPR, m = m0 + wm + j * 32 + row;
-            float v[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; i += 4) {
-                const f32x4 f = *reinterpret_cast<const f32x4*>(&strip[row * OUT_LD + nl + i]);
-                v[i] = f[0] + bv[i]; v[i + 1] = f[1] + bv[i + 1]; v[i + 2] = f[2] + bv[i + 2]; v[i + 3] = f[3] + bv[i + 3];
-            }
-            if (m < X.rows && n < W.rows) store_slot(y + m * ldy, n, W.rows, v);
-        }
-        __builtin_amdgcn_wave_barrier();
-    }
+    mx4_store_tile<T, WM, WN>(reinterpret_cast<float*>(&s0) + wave * 32 * OUT_LD, acc, y, ldy, m0 + wm, n0 + wn, X.rows, W.rows, bias, btype);
 }
 
 // ---- bias gradient: column sums of dy ----------------------------------------------------------------------------------
@@ -470,8 +651,22 @@ static int mx4_check_product(const char* what, const void* x, int64_t ldx, int d
                 "%s: M=%d N=%d, row strides %lld and %lld", what, M, out, (long long)ldx, (long long)ldy);
     return DRM_OK;
 }
-static int mx4_check_grid(const char* what, int M, int rows_per) {
-    DRM_REQUIRE((M + rows_per - 1) / rows_per <= 65535, DRM_ENOTSUP, "%s: M=%d rows (at most %d)", what, M, 65535 * rows_per);
+// Large products: bf16 rows whose 16-byte chunks are aligned and whole go to LDS by direct loads with 128 of the reduction per step;
+// through registers the parts of wider types leave room for 64.
+template <bool GRAD, typename T>
+static void mx4_launch_tile(const T* x, int64_t ldx, const Mx4& W, const void* bias, int btype, T* y, int64_t ldy, int M, int N, int K, hipStream_t s) {
+    const int tm = (M + 127) / 128, tn = (N + 127) / 128;
+    if constexpr (Parts<T>::N == 1) {
+        if (aligned16(x) && ldx % 8 == 0 && K % 8 == 0 && ldx <= (1 << 22)) {
+            k_mx4_tile<T, 128, true, GRAD><<<tm * tn, 256, 0, s>>>(x, ldx, W, bias, btype, y, ldy, M, N, K, tm, tn);
+            return;
+        }
+    }
+    k_mx4_tile<T, Parts<T>::N == 1 ? 128 : 64, false, GRAD><<<tm * tn, 256, 0, s>>>(x, ldx, W, bias, btype, y, ldy, M, N, K, tm, tn);
+}
+static int mx4_check_tiles(const char* what, int M, int N, int K) {
+    DRM_REQUIRE(K <= (1 << 22), DRM_ENOTSUP, "%s: a row of %d elements (at most 4194304)", what, K);
+    DRM_REQUIRE(((int64_t)M + 127) / 128 * (((int64_t)N + 127) / 128) <= INT_MAX / 4, DRM_ENOTSUP, "%s: M=%d N=%d: too many tiles", what, M, N);
     return DRM_OK;
 }
 static inline int mx4_stream_grid(int64_t quads) { return (int)(quads < 256 * 16384ll ? (quads + 255) / 256 : 16384); }
@@ -519,7 +714,7 @@ extern "C" int drm_mx4_linear(const void* x, int64_t ldx, int32_t dtype, const u
     if (M == 0 && N >= 1 && K >= 1) return DRM_OK;
     if (int rc = mx4_check(__func__, codes, scales, N, K)) return rc;
     if (int rc = mx4_check_product(__func__, x, ldx, dtype, K, bias, bias_dtype, y, ldy, N, M)) return rc;
-    if (int rc = mx4_check_grid(__func__, M, 128)) return rc;
+    if (int rc = mx4_check_tiles(__func__, M, N, K)) return rc;
     hipStream_t s = (hipStream_t)stream;
     const Mx4 W{codes, scales, N, mx4_blocks(K)};
     ProfScope ps(M <= 64 ? PC_LINEAR : PC_LINEAR_BIG, s, 2.0 * M * N * K, ((double)M * K + (double)M * N) * elem_bytes(dtype) + (double)N * W.nb * 17);
@@ -529,7 +724,7 @@ extern "C" int drm_mx4_linear(const void* x, int64_t ldx, int32_t dtype, const u
         if (M <= 16) k_mx4_rows<T, 1, 8><<<grid, 512, 0, s>>>((const T*)x, ldx, W, bias, bias_dtype, (T*)y, ldy, M, K);
         else if (M <= 32) k_mx4_rows<T, 2, 8><<<grid, 512, 0, s>>>((const T*)x, ldx, W, bias, bias_dtype, (T*)y, ldy, M, K);
         else if (M <= 64) k_mx4_rows<T, 4, 8><<<grid, 512, 0, s>>>((const T*)x, ldx, W, bias, bias_dtype, (T*)y, ldy, M, K);
-        else k_mx4_tile<T, false><<<dim3((N + 127) / 128, (M + 127) / 128), 256, 0, s>>>((const T*)x, ldx, W, bias, bias_dtype, (T*)y, ldy, M, N, K);
+        else mx4_launch_tile<false, T>((const T*)x, ldx, W, bias, bias_dtype, (T*)y, ldy, M, N, K, s);
         DRM_LAUNCH_CHECK();
         return DRM_OK;
     });
@@ -540,14 +735,14 @@ extern "C" int drm_mx4_linear_dgrad(const void* dy, int64_t lddy, int32_t dtype,
     if (M == 0 && N >= 1 && K >= 1) return DRM_OK;
     if (int rc = mx4_check(__func__, codes, scales, N, K)) return rc;
     if (int rc = mx4_check_product(__func__, dy, lddy, dtype, N, nullptr, 0, dx, lddx, K, M)) return rc;
-    if (int rc = mx4_check_grid(__func__, M, 128)) return rc;
+    if (int rc = mx4_check_tiles(__func__, M, K, K)) return rc;
     DRM_REQUIRE(N >= 1, DRM_EINVAL, "N=%d", N);
     hipStream_t s = (hipStream_t)stream;
     const Mx4 W{codes, scales, N, mx4_blocks(K)};
     ProfScope ps(PC_LINEAR_BIG, s, 2.0 * M * N * K, ((double)M * K + (double)M * N) * elem_bytes(dtype) + (double)N * W.nb * 17);
     return with_elem(dtype, [&](auto tag) -> int {
         using T = decltype(tag);
-        k_mx4_tile<T, true><<<dim3((K + 127) / 128, (M + 127) / 128), 256, 0, s>>>((const T*)dy, lddy, W, nullptr, 0, (T*)dx, lddx, M, K, N);
+        mx4_launch_tile<true, T>((const T*)dy, lddy, W, nullptr, 0, (T*)dx, lddx, M, K, N, s);
         DRM_LAUNCH_CHECK();
         return DRM_OK;
     });
@@ -560,8 +755,7 @@ extern "C" int drm_mx4_product(const uint8_t* x_codes, const uint8_t* x_scales, 
     if (int rc = mx4_check(__func__, x_codes, x_scales, M, K)) return rc;
     if (int rc = mx4_check(__func__, w_codes, w_scales, N, K)) return rc;
     if (int rc = mx4_check_product(__func__, x_codes, K, y_dtype, K, bias, bias_dtype, y, ldy, N, M)) return rc;
-    DRM_REQUIRE(K <= (1 << 22), DRM_ENOTSUP, "K=%d (at most 4194304)", K);
-    DRM_REQUIRE((int64_t)((M + 63) / 64) * ((N + 63) / 64) <= INT_MAX, DRM_ENOTSUP, "M=%d N=%d: too many tiles", M, N);
+    if (int rc = mx4_check_tiles(__func__, M, N, K)) return rc;
     hipStream_t s = (hipStream_t)stream;
     const Mx4 X{x_codes, x_scales, M, mx4_blocks(K)}, W{w_codes, w_scales, N, mx4_blocks(K)};
     ProfScope ps(PC_LINEAR_BIG, s, 2.0 * M * N * K, (double)M * N * elem_bytes(y_dtype) + ((double)M + N) * W.nb * 17);

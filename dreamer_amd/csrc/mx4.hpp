@@ -16,10 +16,8 @@ struct Mx4 {
     int rows, nb;
 };
 
-// scale byte as the fp32 scale operand of the conversion instructions
-__device__ __forceinline__ float mx4_scale(uint32_t s) {
-    return __builtin_bit_cast(float, s == 255u ? 0x7fc00000u : s == 0u ? 0x00400000u : s << 23);
-}
+// scale byte as the scale operand of the conversion instructions: they read its exponent field, 0 as 2^-127 and 255 as NaN
+__device__ __forceinline__ float mx4_scale(uint32_t s) { return __builtin_bit_cast(float, s << 23); }
 
 // eight codes of a block to bf16 (exact: at most two significant bits; below 2^-126 subnormal)
 __device__ __forceinline__ bf16x8 mx4_bf16x8(uint32_t codes, float scale) {
@@ -37,39 +35,40 @@ template <> struct Parts<__bf16> { static constexpr int N = 1; };
 template <> struct Parts<_Float16> { static constexpr int N = 2; };
 template <> struct Parts<float> { static constexpr int N = 3; };
 
+// eight elements as they lie in memory; 0 behind the row
 template <typename T>
-__device__ __forceinline__ void load_parts(const T* __restrict__ row, int64_t at, int64_t len, bf16x8 (&p)[Parts<T>::N]) {
+struct Eight { T v[8]; };
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Packed8 { Eight<T> e; };
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T* __restrict__ row, int64_t at, int64_t len) {
+    if (at + 8 <= len) return reinterpret_cast<const Packed8<T>*>(row + at)->e;
+    Eight<T> r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.v[i] = at + i < len ? row[at + i] : (T)0.f;
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void split_eight(const Eight<T>& e, bf16x8 (&p)[Parts<T>::N]) {
     if constexpr (Parts<T>::N == 1) {
-        if (at + 8 <= len) {
-            p[0] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const Slot<T>*>(row + at));
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) p[0][i] = at + i < len ? row[at + i] : (__bf16)0.f;
-        }
+        p[0] = __builtin_bit_cast(bf16x8, e);
     } else {
-        float v[8];
-        if constexpr (Elem<T>::VEC == 8) {
-            load_slot(row, at, len, 0.f, v);
-        } else {
-            float a[4], b[4];
-            load_slot(row, at, len, 0.f, a);
-            load_slot(row, at + 4, len, 0.f, b);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[i + 4] = b[i]; }
-        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            float x = v[i];
+            float x = (float)e.v[i];
 #pragma unroll
             for (int q = 0; q < Parts<T>::N; ++q) {
                 const uint32_t u = __builtin_bit_cast(uint32_t, x);
-                const uint32_t top = u & 0xffff0000u;
+                const float cut = __builtin_bit_cast(float, u & 0xffff0000u);
                 p[q][i] = __builtin_bit_cast(__bf16, (uint16_t)(u >> 16));
-                const float cut = __builtin_bit_cast(float, top);
-                x = fabsf(cut) == INFINITY && x == cut ? 0.f : x - cut;
+                x = fabsf(x) == INFINITY ? 0.f : x - cut;
             }
         }
     }
+}
+template <typename T>
+__device__ __forceinline__ void load_parts(const T* __restrict__ row, int64_t at, int64_t len, bf16x8 (&p)[Parts<T>::N]) {
+    split_eight<T>(load_eight(row, at, len), p);
 }
 
 }  // namespace drm
