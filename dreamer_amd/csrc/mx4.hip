@@ -1,6 +1,8 @@
 // Microscaled 4-bit floating point: quantisation, its inverse, and the products that read 4-bit weights.
 #include "mx4.hpp"
 
+#include <type_traits>
+
 #include <climits>
 
 namespace drm {
@@ -183,25 +185,30 @@ __device__ __forceinline__ void mx4_store_tile(float* strip, const f32x16 (&acc)
 }
 
 // ---- y = x W^T + bias and dx = dy W, many rows --------------------------------------------------------------------------
-// 128 x 128 outputs per workgroup, four waves of 64 x 64 (32x32x16 bf16 matrix instructions), BK of the reduction per step, two
-// LDS stages.  The float operand lies in LDS in its bf16 parts: rows of BK, 16-byte chunk c of row r at c ^ (r & 7); bf16 rows
+// 128 x 128 outputs per workgroup, eight waves of 64 x 32 (32x32x16 bf16 matrix instructions), BK of the reduction per step, two
+// LDS stages.  Eight waves although four larger ones would read less from LDS: a single wave of a SIMD issues a vector
+// instruction every eight cycles only, two of them every four.  The float operand lies in LDS in its bf16 parts: rows of BK, 16-byte chunks in an order that spreads a fragment's rows over the banks; bf16 rows
 // whose chunks are aligned go there by direct loads, others through registers.
 //   y : the codes lie in LDS as they are and every wave widens the fragments it needs (an eighth of the LDS traffic of
 //       bf16 rows; the conversion instruction takes a quarter of the vector rate, half of the matrix instructions' time).
 //   dx: the reduction runs over W's rows, so that a fragment needs one column of eight rows: the block of a row is widened
 //       once, four rows side by side exchange their dwords (a transposition among four lanes), and the columns go to LDS.
-template <typename T, int BK, bool DIRECT, bool GRAD>
+constexpr int TILE_WAVES = 8, TILE_THREADS = TILE_WAVES * 64;
+template <typename T, int BK, bool GRAD>
 struct TileStage {
     static constexpr int P = Parts<T>::N, NB = BK / 32;
     __attribute__((aligned(16))) uint8_t x[P][128 * BK * 2];
     __attribute__((aligned(16))) uint8_t w[GRAD ? 128 * BK * 2 : 128 * NB * 16];
-    uint32_t sw[GRAD ? 4 : 128];
+    uint32_t sw[GRAD ? 4 : TILE_THREADS];  // 128 rows (brought by every pair of waves)
 };
 
-// position of chunk c in row r of a tile of bf16 rows
-__device__ __forceinline__ int mx4_chunk(int r, int c) { return (c & 8) | ((c ^ r) & 7); }
-// dx: columns of W; eight of them are written by lanes of one instruction, so their number takes part as well
-__device__ __forceinline__ int mx4_chunk_t(int r, int c) { return (c & 8) | ((c ^ r ^ (r >> 3)) & 7); }
+// Position of chunk c in row r of a tile of bf16 rows of CH chunks: the sixteen rows that one clock of a fragment read takes
+// (64 banks, 256 bytes) lie on different banks.  An involution in c.
+template <int CH>
+__device__ __forceinline__ int mx4_chunk(int r, int c) { return CH == 16 ? c ^ (r & 15) : c ^ ((r >> 1) & 7); }
+// dx: columns of W; the lanes of one instruction write columns whose numbers differ by eight, so r / 8 takes part as well
+template <int CH>
+__device__ __forceinline__ int mx4_chunk_t(int r, int c) { return CH == 16 ? c ^ ((r ^ (r >> 3)) & 15) : c ^ (((r >> 1) ^ (r >> 3)) & 7); }
 
 struct __attribute__((packed, aligned(1))) Bytes4 { uint32_t v; };
 struct __attribute__((packed, aligned(1))) Bytes2 { uint16_t v; };
@@ -220,27 +227,27 @@ __device__ __forceinline__ u32x4 quad_transpose(u32x4 d, int q) {
     return d;
 }
 
-template <typename T, int BK, bool DIRECT, bool GRAD>
-__global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64_t ldx, Mx4 W, const void* bias, int btype,
+template <typename T, int BK, bool DIRECT, bool GRAD, bool RING>
+__global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__ x, int64_t ldx, Mx4 W, const void* bias, int btype,
                                                   T* __restrict__ y, int64_t ldy, int M, int N, int K, int tiles_m, int tiles_n) {
     // y: reduction over W's columns (K of them), N = W's rows; dx: reduction over W's rows (K of them), N = W's columns
     static_assert(!DIRECT || Parts<T>::N == 1, "direct loads bring bf16");
-    using Stage = TileStage<T, BK, DIRECT, GRAD>;
-    constexpr int P = Stage::P, NB = Stage::NB, CH = BK / 8, XU = 128 * CH / 256, WU = GRAD ? BK / 64 : 1;
-    constexpr int OUT_LD = 64 + 4;
-    static_assert(sizeof(Stage) >= 4 * 32 * OUT_LD * sizeof(float), "the output strips fit one stage");
+    static_assert(!RING || (DIRECT && !GRAD), "a ring of stages has no loads through registers");
+    using Stage = TileStage<T, BK, GRAD>;
+    constexpr int P = Stage::P, NB = Stage::NB, CH = BK / 8, XU = 128 * CH / TILE_THREADS, WU = GRAD ? BK * 4 / TILE_THREADS + (BK * 4 < TILE_THREADS) : 1;
+    constexpr int WN = 32, OUT_LD = WN + 4;
+    static_assert(sizeof(Stage) >= TILE_WAVES * 32 * OUT_LD * sizeof(float), "the output strips fit one stage");
     __shared__ Stage s0, s1;
+    __shared__ std::conditional_t<RING, Stage, char> s2;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
     int tm, tn;
     mx4_tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
-    const int m0 = tm * 128, n0 = tn * 128, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    f32x16 acc[2][2];
+    const int m0 = tm * 128, n0 = tn * 128, wm = (wave & 1) * 64, wn = (wave >> 1) * WN;
+    f32x16 acc[1][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+        for (int e = 0; e < 16; ++e) acc[0][j][e] = 0.f;
 
     struct Held {                     // what a step brings through registers
         Eight<T> x[DIRECT ? 1 : XU];
@@ -257,7 +264,7 @@ __global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64
         if constexpr (GRAD) {
 #pragma unroll
             for (int j = 0; j < WU; ++j) {
-                const int u = threadIdx.x + 256 * j, n = k0 + (u >> 4) * 4 + (u & 3), kb = (n0 >> 5) + ((u >> 2) & 3);
+                const int u = (threadIdx.x + TILE_THREADS * j) & (BK * 4 - 1), n = k0 + (u >> 4) * 4 + (u & 3), kb = (n0 >> 5) + ((u >> 2) & 3);
                 const int64_t at = (int64_t)min(n, W.rows - 1) * W.nb + min(kb, W.nb - 1);
                 h.sw[j] = W.scales[at];
                 h.w[j] = reinterpret_cast<const u32x4*>(W.codes)[at];
@@ -266,29 +273,28 @@ __global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64
         if constexpr (DIRECT) {
             constexpr int RPI = 64 / CH;                          // rows per wave and instruction
             const int row = lane / CH;
-            const int c = mx4_chunk(row, lane % CH);              // (an involution; rows advance by multiples of RPI)
             const uint8_t* base = reinterpret_cast<const uint8_t*>(x + (int64_t)m0 * ldx + k0);
 #pragma unroll
-            for (int j = 0; j < 128 / RPI / 4; ++j) {
-                const int r = (j * 4 + wave) * RPI + row;
-                const int cc = RPI == 8 ? c : mx4_chunk(r, lane % CH);
+            for (int j = 0; j < 128 / RPI / TILE_WAVES; ++j) {
+                const int r = (j * TILE_WAVES + wave) * RPI + row;
+                const int cc = mx4_chunk<CH>(r, lane % CH);
                 const uint8_t* src = base + (uint32_t)(min(r, M - 1 - m0) * (int)ldx * 2 + cc * 16);
                 src = k0 + cc * 8 < K ? src : reinterpret_cast<const uint8_t*>(&mx4_zero_block);
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src,
-                                                 (__attribute__((address_space(3))) uint32_t*)(st.x[0] + (j * 4 + wave) * 1024), 16, 0, 0);
+                                                 (__attribute__((address_space(3))) uint32_t*)(st.x[0] + (j * TILE_WAVES + wave) * 1024), 16, 0, 0);
             }
         } else {
             // whole chunks of eight; what is left of a row behind them follows in a step of its own
             if (!tail) {
 #pragma unroll
                 for (int j = 0; j < XU; ++j) {
-                    const int u = threadIdx.x + 256 * j, r = u / CH, c = u % CH;
+                    const int u = threadIdx.x + TILE_THREADS * j, r = u / CH, c = u % CH;
                     h.x[j] = reinterpret_cast<const Packed8<T>*>(x + (int64_t)min(m0 + r, M - 1) * ldx + max(min(k0 + c * 8, whole - 8), 0))->e;
                 }
             } else {
 #pragma unroll
                 for (int j = 0; j < XU; ++j) {
-                    const int u = threadIdx.x + 256 * j, r = u / CH, c = u % CH;
+                    const int u = threadIdx.x + TILE_THREADS * j, r = u / CH, c = u % CH;
                     h.x[j] = load_eight(x + (int64_t)min(m0 + r, M - 1) * ldx, k0 + c * 8 < whole ? (int64_t)K : (int64_t)k0 + c * 8, K);
                 }
             }
@@ -296,12 +302,13 @@ __global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64
         if constexpr (!GRAD) {
             const uint8_t* base = W.codes + ((int64_t)n0 * W.nb + (k0 >> 5)) * 16;
 #pragma unroll
-            for (int j = 0; j < NB / 2; ++j) {
-                const int r = (j * 4 + wave) * (64 / NB) + lane / NB, b = mx4_code_slot<NB>(r, lane % NB);
+            for (int j = 0; j < (NB * 2 + TILE_WAVES - 1) / TILE_WAVES; ++j) {
+                if (NB * 2 < TILE_WAVES && wave >= NB * 2) break;      // 64 per step: four waves bring the codes
+                const int r = (j * TILE_WAVES + wave) * (64 / NB) + lane / NB, b = mx4_code_slot<NB>(r, lane % NB);
                 const uint8_t* src = base + (uint32_t)((min(r, N - 1 - n0) * W.nb + b) * 16);
                 src = (k0 >> 5) + b < W.nb ? src : reinterpret_cast<const uint8_t*>(&mx4_zero_block);
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src,
-                                                 (__attribute__((address_space(3))) uint32_t*)(st.w + (j * 4 + wave) * 1024), 16, 0, 0);
+                                                 (__attribute__((address_space(3))) uint32_t*)(st.w + (j * TILE_WAVES + wave) * 1024), 16, 0, 0);
             }
         }
     };
@@ -309,11 +316,11 @@ __global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64
         if constexpr (!DIRECT) {
 #pragma unroll
             for (int j = 0; j < XU; ++j) {
-                const int u = threadIdx.x + 256 * j, r = u / CH, c = u % CH;
+                const int u = threadIdx.x + TILE_THREADS * j, r = u / CH, c = u % CH;
                 bf16x8 p[P];
                 split_eight<T>(tail || k0 + c * 8 < whole ? h.x[j] : Eight<T>{}, p);
 #pragma unroll
-                for (int q = 0; q < P; ++q) *reinterpret_cast<bf16x8*>(st.x[q] + r * BK * 2 + mx4_chunk(r, c) * 16) = p[q];
+                for (int q = 0; q < P; ++q) *reinterpret_cast<bf16x8*>(st.x[q] + r * BK * 2 + mx4_chunk<CH>(r, c) * 16) = p[q];
             }
         }
         if constexpr (!GRAD) {
@@ -322,7 +329,8 @@ __global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64
         } else {
 #pragma unroll
             for (int j = 0; j < WU; ++j) {
-                const int u = threadIdx.x + 256 * j, q = u & 3;
+                const int u = threadIdx.x + TILE_THREADS * j, q = u & 3;
+                if (BK * 4 < TILE_THREADS && u >= BK * 4) break;       // 64 per step: four waves put W away
                 const bool live = k0 + (u >> 4) * 4 + q < W.rows && (n0 >> 5) + ((u >> 2) & 3) < W.nb;
                 const u32x4 d = quad_transpose(live ? h.w[j] : u32x4{0u, 0u, 0u, 0u}, q);
                 const uint32_t own = live ? h.sw[j] : 127u;
@@ -336,28 +344,23 @@ __global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64
                     const uint2 lo = make_uint2(__builtin_amdgcn_perm(r[1][i], r[0][i], 0x05040100u), __builtin_amdgcn_perm(r[3][i], r[2][i], 0x05040100u));
                     const uint2 hi = make_uint2(__builtin_amdgcn_perm(r[1][i], r[0][i], 0x07060302u), __builtin_amdgcn_perm(r[3][i], r[2][i], 0x07060302u));
                     const int c0 = col + 2 * i, c1 = c0 + 1;
-                    *reinterpret_cast<uint2*>(st.w + c0 * BK * 2 + mx4_chunk_t(c0, at >> 3) * 16 + (at & 4) * 2) = lo;
-                    *reinterpret_cast<uint2*>(st.w + c1 * BK * 2 + mx4_chunk_t(c1, at >> 3) * 16 + (at & 4) * 2) = hi;
+                    *reinterpret_cast<uint2*>(st.w + c0 * BK * 2 + mx4_chunk_t<CH>(c0, at >> 3) * 16 + (at & 4) * 2) = lo;
+                    *reinterpret_cast<uint2*>(st.w + c1 * BK * 2 + mx4_chunk_t<CH>(c1, at >> 3) * 16 + (at & 4) * 2) = hi;
                 }
             }
         }
     };
     // A turn (16 of the reduction) fetches the next turn's fragments beside its own matrix instructions: x from LDS, the widened
     // codes of a block that was read a turn earlier.  (y: a lane half holds 16 codes in a row, eight per turn; dx: in order.)
-    struct Turn { bf16x8 a[2], v[P][2]; };
+    struct Turn { bf16x8 a, v[P][2]; };
     auto compute = [&](const Stage& st) {
-        uint32_t sw[2] = {0u, 0u};
-        uint2 q[2][2];
+        uint32_t sw = 0u;
+        uint2 q[2];
         Turn f[2];
-        if constexpr (!GRAD) { sw[0] = st.sw[wn + l32]; sw[1] = st.sw[wn + 32 + l32]; }
+        const int wr = wn + l32;
+        if constexpr (!GRAD) sw = st.sw[wr];
         auto codes = [&](int b) {
-            if constexpr (!GRAD) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int r = wn + i * 32 + l32;
-                    q[b & 1][i] = *reinterpret_cast<const uint2*>(st.w + r * NB * 16 + mx4_code_slot<NB>(r, b) * 16 + half * 8);
-                }
-            }
+            if constexpr (!GRAD) q[b & 1] = *reinterpret_cast<const uint2*>(st.w + wr * NB * 16 + mx4_code_slot<NB>(wr, b) * 16 + half * 8);
         };
         auto fetch = [&](int t) {
             const int b = t >> 1, c = GRAD ? t * 2 + half : b * 4 + half * 2 + (t & 1);
@@ -366,17 +369,10 @@ __global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int r = wm + j * 32 + l32;
-                    f[t & 1].v[p][j] = *reinterpret_cast<const bf16x8*>(st.x[p] + r * BK * 2 + mx4_chunk(r, c) * 16);
+                    f[t & 1].v[p][j] = *reinterpret_cast<const bf16x8*>(st.x[p] + r * BK * 2 + mx4_chunk<CH>(r, c) * 16);
                 }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if constexpr (GRAD) {
-                    const int r = wn + i * 32 + l32;
-                    f[t & 1].a[i] = *reinterpret_cast<const bf16x8*>(st.w + r * BK * 2 + mx4_chunk_t(r, c) * 16);
-                } else {
-                    f[t & 1].a[i] = mx4_bf16x8((t & 1) == 0 ? q[b & 1][i].x : q[b & 1][i].y, mx4_scale((sw[i] >> (8 * b)) & 255u));
-                }
-            }
+            if constexpr (GRAD) f[t & 1].a = *reinterpret_cast<const bf16x8*>(st.w + wr * BK * 2 + mx4_chunk_t<CH>(wr, c) * 16);
+            else f[t & 1].a = mx4_bf16x8((t & 1) == 0 ? q[b & 1].x : q[b & 1].y, mx4_scale((sw >> (8 * b)) & 255u));
         };
         codes(0);
         fetch(0);
@@ -388,12 +384,10 @@ __global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64
 #pragma unroll
             for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int j = 0; j < 2; ++j)
+                    acc[0][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[t & 1].a, f[t & 1].v[p][j], acc[0][j], 0, 0, 0);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[t & 1].a[i], f[t & 1].v[p][j], acc[i][j], 0, 0, 0);
-#pragma unroll
-            for (int k = 0; k < 4 * P; ++k) {
+            for (int k = 0; k < 2 * P; ++k) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
                 __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
@@ -402,7 +396,7 @@ __global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64
         }
     };
     Held h;
-    if constexpr (!GRAD) {
+    if constexpr (!GRAD && !RING) {
         if (W.nb >= NB) {
             load_scales(0, h);
         } else {                          // a row shorter than a step (then there is no second one)
@@ -412,7 +406,40 @@ __global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64
         }
     }
     const int steps = (whole + BK - 1) / BK;
-    if (steps > 0) {
+    if constexpr (RING) {
+        // Three stages, filled by direct loads only (rows of whole steps of blocks: every row's four scale bytes of a step are an
+        // aligned dword).  Stage i's loads are issued two steps ahead.  Before it is used, every wave waits until no more than the next
+        // stage's loads are under way (fences keep the loads of a stage together) and meets the others; behind that barrier the
+        // stage of the step before is free for new loads.
+        constexpr int AHEAD = 128 * CH / TILE_THREADS + NB * 2 / TILE_WAVES + 1;
+        static_assert(NB * 2 % TILE_WAVES == 0, "every wave brings as much");
+        auto issue = [&](Stage& st, int k0) {
+            asm volatile("" ::: "memory");
+            const int kb0 = min(k0 >> 5, W.nb - NB);          // behind the last step: anything inside the row
+            const uint8_t* src = W.scales + (int64_t)min(n0 + (int)(threadIdx.x & 127), N - 1) * W.nb + kb0;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src,
+                                             (__attribute__((address_space(3))) uint32_t*)(st.sw + wave * 64), 4, 0, 0);
+            load(st, k0, h, false);
+            asm volatile("" ::: "memory");
+        };
+        auto turn = [&](Stage& st, int k0, Stage& after) {
+            __builtin_amdgcn_s_waitcnt((AHEAD & 15) | (AHEAD >> 4) << 14 | 0x0070);      // vmcnt(AHEAD), lgkmcnt(0)
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            issue(after, k0 + 2 * BK);
+            compute(st);
+        };
+        issue(s0, 0);
+        issue(s1, BK);
+        int k0 = 0;
+        for (int p = 0; p < steps / 3; ++p, k0 += 3 * BK) {
+            turn(s0, k0, s2);
+            turn(s1, k0 + BK, s0);
+            turn(s2, k0 + 2 * BK, s1);
+        }
+        if (steps % 3 > 0) turn(s0, k0, s2);
+        if (steps % 3 > 1) turn(s1, k0 + BK, s0);
+    } else if (steps > 0) {
         load(s0, 0, h, false);
         put(s0, 0, h, false);
         __syncthreads();
@@ -440,14 +467,14 @@ __global__ __launch_bounds__(256) void k_mx4_tile(const T* __restrict__ x, int64
         compute(s1);
     }
     __syncthreads();
-    mx4_store_tile<T, 64, 64>(reinterpret_cast<float*>(&s0) + wave * 32 * OUT_LD, acc, y, ldy, m0 + wm, n0 + wn, M, N, bias, btype);
+    mx4_store_tile<T, 64, WN>(reinterpret_cast<float*>(&s0) + wave * 32 * OUT_LD, acc, y, ldy, m0 + wm, n0 + wn, M, N, bias, btype);
 }
 
 // ---- both operands in 4 bits ----------------------------------------------------------------------------------------------
 // Tiles of BM x BN outputs, 256 deep per step (eight blocks, 128 bytes a row), four waves, each owning WM x WN of 32x32x64 scaled
 // matrix instructions.  The codes go from memory to LDS as they are (16-byte direct loads, no registers in between), two buffers:
 // the loads of the next step run under the matrix instructions of this one.  A direct load fills LDS in lane order, so the lanes
-// choose their source instead: slot p of row r holds block p ^ (r & 7), and the 32 rows a fragment read touches fall on all banks.
+// choose their source instead: slot p of row r holds block p ^ (r / 2 & 7): a fragment read takes 16 rows a clock, which then fall on all 64 banks.
 // An instruction's lane half h takes block 4 h + s of the step's eight in its s-th turn -- a permutation of the reduction index that
 // both operands share -- so that one dword holds a lane's four scales and the turn selects the byte.
 // Blocks behind the last one come from the zero block, rows behind the last one repeat it and are not stored.
@@ -466,7 +493,7 @@ __device__ __forceinline__ void mx4_stage_codes(const Mx4& A, int r0, int kb0, u
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int lr = wave * 8 + (lane >> 3);
     asm volatile("" : "+v"(lr));            // offsets are formed at each step: kept, they would take the accumulators' registers
-    const int c = (lane & 7) ^ (lane >> 3), last = A.rows - 1 - r0;
+    const int c = (lane & 7) ^ (((wave * 8 + (lane >> 3)) >> 1) & 7), last = A.rows - 1 - r0;
     const uint8_t* base = A.codes + ((int64_t)r0 * A.nb + kb0) * 16;      // offsets inside a tile stay below 2^31 (checked at the call)
 #pragma unroll
     for (int j = 0; j < ROWS / 32; ++j) {
@@ -498,7 +525,7 @@ __device__ __forceinline__ uint2 mx4_short_row_scales(const Mx4& A, int row) {
 template <int S, int TM, int TN>
 __device__ __forceinline__ void mx4_turn_load(const uint8_t* x, const uint8_t* w, u32x4 (&b)[TM], u32x4 (&a)[TN]) {
     const int lane = threadIdx.x & 63;
-    const int at = (lane & 31) * 128 + ((((lane >> 5) * 4 + S) ^ (lane & 7)) * 16);
+    const int at = (lane & 31) * 128 + ((((lane >> 5) * 4 + S) ^ ((lane >> 1) & 7)) * 16);
 #pragma unroll
     for (int i = 0; i < TN; ++i) a[i] = *reinterpret_cast<const u32x4*>(w + i * 32 * 128 + at);
 #pragma unroll
@@ -651,18 +678,24 @@ static int mx4_check_product(const char* what, const void* x, int64_t ldx, int d
                 "%s: M=%d N=%d, row strides %lld and %lld", what, M, out, (long long)ldx, (long long)ldy);
     return DRM_OK;
 }
-// Large products: bf16 rows whose 16-byte chunks are aligned and whole go to LDS by direct loads with 128 of the reduction per step;
-// through registers the parts of wider types leave room for 64.
+// Large products: bf16 rows whose 16-byte chunks are aligned and whole go to LDS by direct loads with 128 of the reduction per step
+// (three stages where a row's scales are whole dwords); through registers the parts of wider types leave room for 64.
 template <bool GRAD, typename T>
 static void mx4_launch_tile(const T* x, int64_t ldx, const Mx4& W, const void* bias, int btype, T* y, int64_t ldy, int M, int N, int K, hipStream_t s) {
     const int tm = (M + 127) / 128, tn = (N + 127) / 128;
     if constexpr (Parts<T>::N == 1) {
         if (aligned16(x) && ldx % 8 == 0 && K % 8 == 0 && ldx <= (1 << 22)) {
-            k_mx4_tile<T, 128, true, GRAD><<<tm * tn, 256, 0, s>>>(x, ldx, W, bias, btype, y, ldy, M, N, K, tm, tn);
+            if constexpr (!GRAD) {
+                if (W.nb % 4 == 0 && ((uintptr_t)W.scales & 3) == 0) {
+                    k_mx4_tile<T, 128, true, false, true><<<tm * tn, TILE_THREADS, 0, s>>>(x, ldx, W, bias, btype, y, ldy, M, N, K, tm, tn);
+                    return;
+                }
+            }
+            k_mx4_tile<T, 128, true, GRAD, false><<<tm * tn, TILE_THREADS, 0, s>>>(x, ldx, W, bias, btype, y, ldy, M, N, K, tm, tn);
             return;
         }
     }
-    k_mx4_tile<T, Parts<T>::N == 1 ? 128 : 64, false, GRAD><<<tm * tn, 256, 0, s>>>(x, ldx, W, bias, btype, y, ldy, M, N, K, tm, tn);
+    k_mx4_tile<T, Parts<T>::N == 1 ? 128 : 64, false, GRAD, false><<<tm * tn, TILE_THREADS, 0, s>>>(x, ldx, W, bias, btype, y, ldy, M, N, K, tm, tn);
 }
 static int mx4_check_tiles(const char* what, int M, int N, int K) {
     DRM_REQUIRE(K <= (1 << 22), DRM_ENOTSUP, "%s: a row of %d elements (at most 4194304)", what, K);
