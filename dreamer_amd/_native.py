@@ -5,8 +5,8 @@ wrappers, and every wrapper raises if the shared object is missing or a call fai
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
+import functools
 import os
 from typing import Optional
 
@@ -734,85 +734,122 @@ def prof_summary():
 
 
 # --------------------------------------------------------------------------- operators on fp32, bf16 and fp16 tensors
+# A small call costs what its host side costs, so these wrappers look things up once, allocate as little as they can and read
+# the current device and stream from torch's own accessors.
 DTYPE_ID = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_get_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def on_device(device):
-    """Context in which ``device`` is the current one: kernels are launched on the device that is current (a no-op when it is)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _launch(name: str, device: int, *args) -> None:
+    """Call an entry point whose last argument is the stream, on ``device`` (kernels go to the device that is current)."""
+    fn = getattr(_lib or lib(), name)
+    if _get_device() == device:
+        rc = fn(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(device))
+    if rc != 0:
+        check(rc, name)
+
+
+def _device_of(ref: torch.Tensor, **others) -> int:
+    device = ref.get_device()
+    if device < 0:
+        raise NativeError("this operation runs only on a HIP device tensor")
+    for name, t in others.items():
+        if t is not None and t.get_device() != device:
+            raise NativeError(f"{name} is on {t.device}, the operation runs on {ref.device}")
+    return device
 
 
 def dtype_id(t: torch.Tensor, name: str) -> int:
-    if t.dtype not in DTYPE_ID:
+    i = DTYPE_ID.get(t.dtype)
+    if i is None:
         raise NativeError(f"{name}: expected fp32, bf16 or fp16, got {t.dtype}")
-    return DTYPE_ID[t.dtype]
-
-
-def same_device(ref: torch.Tensor, **others) -> None:
-    if not ref.is_cuda:
-        raise NativeError("this operation runs only on a HIP device tensor")
-    for name, t in others.items():
-        if t is not None and t.device != ref.device:
-            raise NativeError(f"{name} is on {t.device}, the operation runs on {ref.device}")
+    return i
 
 
 def as_rows(x: torch.Tensor) -> torch.Tensor:
     """x as a matrix over its last dimension whose columns are contiguous and whose rows do not overlap (a view where it can be)."""
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    return x2 if x2.stride(1) == 1 and x2.stride(0) >= x2.shape[1] else x2.contiguous()
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    if x.is_contiguous():
+        return x
+    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
+
+
+def _row_stride(x: torch.Tensor) -> int:
+    """Distance of a matrix's rows (a single row's stride is arbitrary and not used)."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(name: str, *sizes: int) -> int:
+    return getattr(lib(), name)(*sizes)
+
+
+def _workspace(device, name: str, *sizes: int):
+    need = _workspace_bytes(name, *sizes)
+    return (torch.empty(need // 4, dtype=torch.float32, device=device), need) if need else (None, 0)
 
 
 def layer_norm_forward(x, weight, bias, eps: float, want_stats: bool):
-    """LayerNorm over the rows of x (N, E); returns y (dense), mean (N), rstd (N) (None without ``want_stats``)."""
-    same_device(x, weight=weight, bias=bias)
+    """LayerNorm over the rows of x (N, E); returns y (dense) and the rows' (mean, rstd) as (2, N) (None without ``want_stats``)."""
     xid = dtype_id(x, "x")
+    device = _device_of(x, weight=weight, bias=bias)
     N, E = x.shape
-    wid = xid
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            wid = dtype_id(t, name)
-            if t.shape != (E,) or not t.is_contiguous():
-                raise NativeError(f"layer_norm: {name} has shape {tuple(t.shape)}, rows have {E} elements")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise NativeError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
+    wid, wp, bp = xid, None, None
+    if weight is not None:
+        wid, wp = dtype_id(weight, "weight"), weight.data_ptr()
+        if weight.shape != (E,) or not weight.is_contiguous():
+            raise NativeError(f"layer_norm: weight has shape {tuple(weight.shape)}, rows have {E} elements")
+    if bias is not None:
+        if weight is not None and weight.dtype != bias.dtype:
+            raise NativeError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
+        wid, bp = dtype_id(bias, "bias"), bias.data_ptr()
+        if bias.shape != (E,) or not bias.is_contiguous():
+            raise NativeError(f"layer_norm: bias has shape {tuple(bias.shape)}, rows have {E} elements")
     y = torch.empty((N, E), dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, N), dtype=torch.float32, device=x.device) if want_stats else None
-    mean, rstd = (stats[0], stats[1]) if want_stats else (None, None)
-    with on_device(x.device):
-        check(lib().drm_layer_norm_forward(x.data_ptr(), x.stride(0), xid, ptr(weight), ptr(bias), wid, y.data_ptr(), E, ptr(mean), ptr(rstd),
-                                           N, E, float(eps), stream_ptr(x.device)), "drm_layer_norm_forward")
-    return y, mean, rstd
+    stats = mean = rstd = None
+    if want_stats:
+        stats = torch.empty((2, N), dtype=torch.float32, device=x.device)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * N
+    if N:
+        _launch("drm_layer_norm_forward", device, x.data_ptr(), _row_stride(x), xid, wp, bp, wid, y.data_ptr(), E, mean, rstd, N, E, eps)
+    return y, stats
 
 
-def layer_norm_backward(x, dy, weight, mean, rstd, want_dx: bool, dw_dtype, db_dtype):
-    """dx (N, E), d weight, d bias (E) of layer_norm_forward; a result whose flag / dtype is False / None is not formed."""
-    same_device(x, dy=dy, weight=weight, mean=mean, rstd=rstd)
+def layer_norm_backward(x, dy, weight, stats, want_dx: bool, want_dw: bool, want_db: bool, bias_dtype=None):
+    """dx (N, E), d weight, d bias (E) of layer_norm_forward; None for a result that is not wanted."""
     xid = dtype_id(x, "x")
+    device = _device_of(x, dy=dy, weight=weight, stats=stats)
     N, E = x.shape
-    if dy.shape != x.shape or dy.dtype != x.dtype or mean.numel() != N or rstd.numel() != N:
+    if dy.shape != x.shape or dy.dtype != x.dtype or stats.shape != (2, N) or stats.dtype != torch.float32 or not stats.is_contiguous():
         raise NativeError(f"layer_norm_backward: gradient {tuple(dy.shape)} {dy.dtype} does not match rows {tuple(x.shape)} {x.dtype}")
     if weight is not None and (weight.shape != (E,) or not weight.is_contiguous()):
         raise NativeError(f"layer_norm_backward: weight has shape {tuple(weight.shape)}, rows have {E} elements")
-    wdtype = weight.dtype if weight is not None else (db_dtype or x.dtype)
-    if any(d is not None and d != wdtype for d in (dw_dtype, db_dtype)):
-        raise NativeError("layer_norm_backward: the weight's and the bias's gradient have the weight's type")
-    dx = torch.empty((N, E), dtype=x.dtype, device=x.device) if want_dx else None
-    dw = torch.empty(E, dtype=wdtype, device=x.device) if dw_dtype is not None else None
-    db = torch.empty(E, dtype=wdtype, device=x.device) if db_dtype is not None else None
-    need = lib().drm_layer_norm_workspace_bytes(N, E)
-    ws = torch.empty(need // 4, dtype=torch.float32, device=x.device)
-    with on_device(x.device):
-        check(lib().drm_layer_norm_backward(x.data_ptr(), x.stride(0), dy.data_ptr(), dy.stride(0), xid, ptr(weight), DTYPE_ID[wdtype],
-                                            mean.data_ptr(), rstd.data_ptr(), ptr(dx), ptr(dw), ptr(db), N, E, ws.data_ptr(), need,
-                                            stream_ptr(x.device)), "drm_layer_norm_backward")
+    if (want_dw and weight is None) or (want_db and bias_dtype is None) or (weight is not None and want_db and bias_dtype != weight.dtype):
+        raise NativeError("layer_norm_backward: a gradient of a weight that is not there, or weight and bias of different types")
+    wdtype = weight.dtype if weight is not None else (bias_dtype or x.dtype)
+    dev = x.device
+    dx = torch.empty((N, E), dtype=x.dtype, device=dev) if want_dx else None
+    dw = torch.empty(E, dtype=wdtype, device=dev) if want_dw else None
+    db = torch.empty(E, dtype=wdtype, device=dev) if want_db else None
+    ws, need = _workspace(dev, "drm_layer_norm_workspace_bytes", N, E)
+    mean = stats.data_ptr()
+    _launch("drm_layer_norm_backward", device, x.data_ptr(), _row_stride(x), dy.data_ptr(), _row_stride(dy), xid, ptr(weight), DTYPE_ID[wdtype],
+            mean, mean + 4 * N, ptr(dx), ptr(dw), ptr(db), N, E, ptr(ws), need)
     return dx, dw, db
 
 
 def distill_topk_forward(logits, top_values, top_indices, top_lse, temperature: float):
     """Loss rows (rows,) of the student logits (rows, V) against the listed teacher entries (rows, k), and what
     ``distill_topk_backward`` takes: p (rows, k) and the row factors (rows, 4)."""
-    same_device(logits, top_values=top_values, top_indices=top_indices, top_lse=top_lse)
     lid = dtype_id(logits, "logits")
+    device = _device_of(logits, top_values=top_values, top_indices=top_indices, top_lse=top_lse)
     rows, V = logits.shape
     k = top_indices.shape[1]
     if top_values.shape != (rows, k) or top_indices.shape != (rows, k) or (top_lse is not None and top_lse.shape != (rows,)):
@@ -820,81 +857,78 @@ def distill_topk_forward(logits, top_values, top_indices, top_lse, temperature: 
                           + (f", top_lse {tuple(top_lse.shape)}" if top_lse is not None else ""))
     if top_values.dtype != torch.float32 or top_indices.dtype != torch.int64 or (top_lse is not None and top_lse.dtype != torch.float32):
         raise NativeError("distill_topk: top_values and top_lse must be fp32, top_indices int64")
-    if k and (top_values.stride(1) != 1 or top_indices.stride(1) != 1):
-        raise NativeError("distill_topk: lists need contiguous rows")
-    if top_lse is not None:
-        _dense(top_lse, torch.float32, "top_lse")
-    loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    p = torch.empty((rows, k), dtype=torch.float32, device=logits.device)
-    row = torch.empty((rows, 4), dtype=torch.float32, device=logits.device)
-    need = lib().drm_distill_topk_workspace_bytes(rows, V)
-    ws = torch.empty(need // 4, dtype=torch.float32, device=logits.device) if need else None
-    with on_device(logits.device):
-        check(lib().drm_distill_topk_forward(logits.data_ptr(), logits.stride(0), lid, top_values.data_ptr(), top_values.stride(0),
-                                             top_indices.data_ptr(), top_indices.stride(0), ptr(top_lse), rows, V, k, float(temperature),
-                                             loss.data_ptr(), p.data_ptr(), row.data_ptr(), ptr(ws), need, stream_ptr(logits.device)),
-              "drm_distill_topk_forward")
+    if not (top_values.is_contiguous() and top_indices.is_contiguous() and (top_lse is None or top_lse.is_contiguous())):
+        raise NativeError("distill_topk: the lists must be contiguous")
+    dev = logits.device
+    loss = torch.empty(rows, dtype=torch.float32, device=dev)
+    p = torch.empty((rows, k), dtype=torch.float32, device=dev)
+    row = torch.empty((rows, 4), dtype=torch.float32, device=dev)
+    if rows:
+        ws, need = _workspace(dev, "drm_distill_topk_workspace_bytes", rows, V)
+        _launch("drm_distill_topk_forward", device, logits.data_ptr(), _row_stride(logits), lid, top_values.data_ptr(), k, top_indices.data_ptr(), k,
+                ptr(top_lse), rows, V, k, temperature, loss.data_ptr(), p.data_ptr(), row.data_ptr(), ptr(ws), need)
     return loss, p, row
 
 
 def distill_topk_backward(logits, top_indices, p, row, g_rows, temperature: float) -> torch.Tensor:
     """Gradient wrt the student logits (rows, V), dense, in the logits' type."""
-    same_device(logits, top_indices=top_indices, p=p, row=row, g_rows=g_rows)
     lid = dtype_id(logits, "logits")
+    device = _device_of(logits, top_indices=top_indices, p=p, row=row, g_rows=g_rows)
     rows, V = logits.shape
     k = p.shape[1]
     _dense(p, torch.float32, "p"); _dense(row, torch.float32, "row"); _dense(g_rows, torch.float32, "g_rows")
     if p.shape[0] != rows or row.shape != (rows, 4) or g_rows.numel() != rows or top_indices.shape != (rows, k) \
-            or top_indices.dtype != torch.int64 or (k and top_indices.stride(1) != 1):
+            or top_indices.dtype != torch.int64 or not top_indices.is_contiguous():
         raise NativeError(f"distill_topk_backward: operands do not match {rows} rows with {k} listed entries")
     d = torch.empty((rows, V), dtype=logits.dtype, device=logits.device)
-    with on_device(logits.device):
-        check(lib().drm_distill_topk_backward(logits.data_ptr(), logits.stride(0), lid, top_indices.data_ptr(), top_indices.stride(0),
-                                              p.data_ptr(), row.data_ptr(), g_rows.data_ptr(), rows, V, k, float(temperature), d.data_ptr(),
-                                              stream_ptr(logits.device)), "drm_distill_topk_backward")
+    if rows:
+        _launch("drm_distill_topk_backward", device, logits.data_ptr(), _row_stride(logits), lid, top_indices.data_ptr(), k, p.data_ptr(),
+                row.data_ptr(), g_rows.data_ptr(), rows, V, k, temperature, d.data_ptr())
     return d
 
 
 def mx4_quantize(x: torch.Tensor):
     """codes (rows, nb * 16) and scales (rows, nb) uint8 of a float matrix (rows, K), nb = ceil(K / 32)."""
-    same_device(x)
     xid = dtype_id(x, "x")
+    device = _device_of(x)
     rows, K = x.shape
     nb = (K + 31) // 32
     codes = torch.empty((rows, nb * 16), dtype=torch.uint8, device=x.device)
     scales = torch.empty((rows, nb), dtype=torch.uint8, device=x.device)
-    with on_device(x.device):
-        check(lib().drm_mx4_quantize(x.data_ptr(), x.stride(0), xid, rows, K, codes.data_ptr(), scales.data_ptr(), stream_ptr(x.device)),
-              "drm_mx4_quantize")
+    if rows:
+        _launch("drm_mx4_quantize", device, x.data_ptr(), _row_stride(x), xid, rows, K, codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
 def mx4_dequantize(codes, scales, K: int, dtype) -> torch.Tensor:
-    _mx4_operand(codes, scales, K, "mx4_dequantize")
-    if dtype not in DTYPE_ID:
+    """The values (rows, K) of a 4-bit matrix."""
+    device = _mx4_operand(codes, scales, K, "mx4_dequantize")
+    did = DTYPE_ID.get(dtype)
+    if did is None:
         raise NativeError(f"mx4_dequantize: expected fp32, bf16 or fp16, got {dtype}")
     rows = codes.shape[0]
     y = torch.empty((rows, K), dtype=dtype, device=codes.device)
-    with on_device(codes.device):
-        check(lib().drm_mx4_dequantize(codes.data_ptr(), scales.data_ptr(), rows, K, y.data_ptr(), K, DTYPE_ID[dtype], stream_ptr(codes.device)),
-              "drm_mx4_dequantize")
+    if rows:
+        _launch("drm_mx4_dequantize", device, codes.data_ptr(), scales.data_ptr(), rows, K, y.data_ptr(), K, did)
     return y
 
 
-def _mx4_operand(codes, scales, K: int, what: str) -> None:
-    same_device(codes, scales=scales)
+def _mx4_operand(codes, scales, K: int, what: str) -> int:
+    device = _device_of(codes, scales=scales)
     _dense(codes, torch.uint8, "codes"); _dense(scales, torch.uint8, "scales")
     nb = (K + 31) // 32
-    if K < 1 or codes.dim() != 2 or tuple(codes.shape) != (scales.shape[0], nb * 16) or scales.dim() != 2 or scales.shape[1] != nb:
+    if K < 1 or codes.dim() != 2 or codes.shape != (scales.shape[0], nb * 16) or scales.shape != (codes.shape[0], nb):
         raise NativeError(f"{what}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not a 4-bit matrix of {K} columns")
     if codes.data_ptr() % 16:
         raise NativeError(f"{what}: codes must be 16-byte aligned")
+    return device
 
 
-def _mx4_bias(bias, N: int, ref: torch.Tensor, what: str) -> int:
+def _mx4_bias(bias, N: int, device: int, what: str) -> int:
     if bias is None:
         return 0
-    same_device(ref, bias=bias)
+    if bias.get_device() != device:
+        raise NativeError(f"bias is on {bias.device}, the operation runs on cuda:{device}")
     if bias.shape != (N,) or not bias.is_contiguous():
         raise NativeError(f"{what}: bias has shape {tuple(bias.shape)}, the weight has {N} rows")
     return dtype_id(bias, "bias")
@@ -902,64 +936,58 @@ def _mx4_bias(bias, N: int, ref: torch.Tensor, what: str) -> int:
 
 def mx4_linear(x, codes, scales, bias=None) -> torch.Tensor:
     """x (M, K) @ W.T + bias for a 4-bit weight W (N, K); the result has x's type."""
-    same_device(x, codes=codes)
     xid = dtype_id(x, "x")
     M, K = x.shape
-    _mx4_operand(codes, scales, K, "mx4_linear")
+    device = _mx4_operand(codes, scales, K, "mx4_linear")
+    _device_of(x, codes=codes)
     N = codes.shape[0]
-    bid = _mx4_bias(bias, N, x, "mx4_linear")
+    bid = _mx4_bias(bias, N, device, "mx4_linear")
     y = torch.empty((M, N), dtype=x.dtype, device=x.device)
     if M and N:
-        with on_device(x.device):
-            check(lib().drm_mx4_linear(x.data_ptr(), x.stride(0), xid, codes.data_ptr(), scales.data_ptr(), ptr(bias), bid, y.data_ptr(), N, M,
-                                       N, K, stream_ptr(x.device)), "drm_mx4_linear")
+        _launch("drm_mx4_linear", device, x.data_ptr(), _row_stride(x), xid, codes.data_ptr(), scales.data_ptr(), ptr(bias), bid, y.data_ptr(), N,
+                M, N, K)
     return y
 
 
 def mx4_linear_dgrad(dy, codes, scales, K: int) -> torch.Tensor:
     """dy (M, N) @ W for a 4-bit weight W (N, K): the input gradient of ``mx4_linear``, in dy's type."""
-    same_device(dy, codes=codes)
     yid = dtype_id(dy, "dy")
-    _mx4_operand(codes, scales, K, "mx4_linear_dgrad")
+    device = _mx4_operand(codes, scales, K, "mx4_linear_dgrad")
+    _device_of(dy, codes=codes)
     M, N = dy.shape
     if codes.shape[0] != N:
         raise NativeError(f"mx4_linear_dgrad: gradient has {N} columns, the weight {codes.shape[0]} rows")
     dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
     if M and N:
-        with on_device(dy.device):
-            check(lib().drm_mx4_linear_dgrad(dy.data_ptr(), dy.stride(0), yid, codes.data_ptr(), scales.data_ptr(), dx.data_ptr(), K, M, N, K,
-                                             stream_ptr(dy.device)), "drm_mx4_linear_dgrad")
+        _launch("drm_mx4_linear_dgrad", device, dy.data_ptr(), _row_stride(dy), yid, codes.data_ptr(), scales.data_ptr(), dx.data_ptr(), K, M, N, K)
     return dx if N else dx.zero_()
 
 
 def mx4_bias_grad(dy, dtype) -> torch.Tensor:
     """Column sums of dy (M, N) in ``dtype``, added in fp32 in an order that depends on the shape only."""
-    same_device(dy)
     yid = dtype_id(dy, "dy")
+    device = _device_of(dy)
     M, N = dy.shape
     db = torch.empty(N, dtype=dtype, device=dy.device)
     if not M or not N:
         return db.zero_()
-    need = lib().drm_mx4_bias_grad_workspace_bytes(M, N)
-    ws = torch.empty(need // 4, dtype=torch.float32, device=dy.device)
-    with on_device(dy.device):
-        check(lib().drm_mx4_bias_grad(dy.data_ptr(), dy.stride(0), yid, db.data_ptr(), DTYPE_ID[dtype], M, N, ws.data_ptr(), need,
-                                      stream_ptr(dy.device)), "drm_mx4_bias_grad")
+    ws, need = _workspace(dy.device, "drm_mx4_bias_grad_workspace_bytes", M, N)
+    _launch("drm_mx4_bias_grad", device, dy.data_ptr(), _row_stride(dy), yid, db.data_ptr(), DTYPE_ID[dtype], M, N, ptr(ws), need)
     return db
 
 
 def mx4_product(x_codes, x_scales, w_codes, w_scales, K: int, bias, dtype) -> torch.Tensor:
     """X (M, K) @ W.T + bias with both operands in 4 bits, the result in ``dtype``."""
-    _mx4_operand(x_codes, x_scales, K, "mx4_product")
+    device = _mx4_operand(x_codes, x_scales, K, "mx4_product")
     _mx4_operand(w_codes, w_scales, K, "mx4_product")
-    same_device(x_codes, weight=w_codes)
-    if dtype not in DTYPE_ID:
+    _device_of(x_codes, weight=w_codes)
+    did = DTYPE_ID.get(dtype)
+    if did is None:
         raise NativeError(f"mx4_product: expected fp32, bf16 or fp16, got {dtype}")
     M, N = x_codes.shape[0], w_codes.shape[0]
-    bid = _mx4_bias(bias, N, x_codes, "mx4_product")
+    bid = _mx4_bias(bias, N, device, "mx4_product")
     y = torch.empty((M, N), dtype=dtype, device=x_codes.device)
     if M and N:
-        with on_device(x_codes.device):
-            check(lib().drm_mx4_product(x_codes.data_ptr(), x_scales.data_ptr(), w_codes.data_ptr(), w_scales.data_ptr(), ptr(bias), bid,
-                                        y.data_ptr(), N, DTYPE_ID[dtype], M, N, K, stream_ptr(x_codes.device)), "drm_mx4_product")
+        _launch("drm_mx4_product", device, x_codes.data_ptr(), x_scales.data_ptr(), w_codes.data_ptr(), w_scales.data_ptr(), ptr(bias), bid,
+                y.data_ptr(), N, did, M, N, K)
     return y

@@ -699,6 +699,7 @@ static void mx4_launch_tile(const T* x, int64_t ldx, const Mx4& W, const void* b
 }
 static int mx4_check_tiles(const char* what, int M, int N, int K) {
     DRM_REQUIRE(K <= (1 << 22), DRM_ENOTSUP, "%s: a row of %d elements (at most 4194304)", what, K);
+    DRM_REQUIRE(M <= 65535 * 128, DRM_ENOTSUP, "%s: M=%d rows (at most %d)", what, M, 65535 * 128);
     DRM_REQUIRE(((int64_t)M + 127) / 128 * (((int64_t)N + 127) / 128) <= INT_MAX / 4, DRM_ENOTSUP, "%s: M=%d N=%d: too many tiles", what, M, N);
     return DRM_OK;
 }

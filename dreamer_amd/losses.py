@@ -107,6 +107,14 @@ def critic_loss_rows(logits: torch.Tensor, slow_logits, returns: torch.Tensor, b
                                    returns.detach().reshape(-1).float().contiguous(), float(bucket_min), float(bucket_max), float(reg))
 
 
+def _distill_grad(ctx, g):
+    logits, top_indices, p, row = ctx.saved_tensors
+    return N.distill_topk_backward(logits, top_indices, p, row, g.contiguous(), ctx.temperature), None, None, None, None
+
+
+_distill_grad_once = once_differentiable(_distill_grad)
+
+
 class _DistillTopkRowsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_values, top_indices, top_lse, temperature):
@@ -116,10 +124,17 @@ class _DistillTopkRowsFn(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
-        logits, top_indices, p, row = ctx.saved_tensors
-        return N.distill_topk_backward(logits, top_indices, p, row, g.contiguous(), ctx.temperature), None, None, None, None
+        # (the wrapper that refuses a second differentiation is only needed where one could follow)
+        return _distill_grad_once(ctx, g) if torch.is_grad_enabled() else _distill_grad(ctx, g)
+
+
+def _list_of(t: torch.Tensor, dtype, rows: int, k: int) -> torch.Tensor:
+    """A list (rows, k), dense, in ``dtype``; the tensor itself where it is that."""
+    t = t.detach() if t.requires_grad else t
+    if t.dtype == dtype and t.dim() == 2 and t.is_contiguous():
+        return t
+    return t.to(dtype).reshape(rows, k).contiguous()
 
 
 def _distill_topk_rows_host(s, values, idx, lse, temperature):
@@ -169,8 +184,7 @@ def distill_topk_rows(logits: torch.Tensor, top_values: torch.Tensor, top_indice
         raise N.NativeError(f"distill_topk_rows: top_lse {tuple(top_lse.shape)} does not match logits {tuple(logits.shape)}")
     k = top_indices.shape[-1]
     rows = logits.numel() // logits.shape[-1]
-    values = top_values.detach().float().reshape(rows, k).contiguous()
-    indices = top_indices.long().reshape(rows, k).contiguous()
+    values, indices = _list_of(top_values, torch.float32, rows, k), _list_of(top_indices, torch.int64, rows, k)
     lse = None if top_lse is None else top_lse.detach().float().reshape(-1).contiguous()
     if logits.is_cuda:
         return _DistillTopkRowsFn.apply(N.as_rows(logits), values, indices, lse, float(temperature))

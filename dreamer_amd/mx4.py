@@ -30,6 +30,13 @@ class MX4Tensor:
         N._mx4_operand(codes, scales, int(columns), "MX4Tensor")
         self.codes, self.scales, self.columns = codes, scales, int(columns)
 
+    @classmethod
+    def _of(cls, codes: torch.Tensor, scales: torch.Tensor, columns: int) -> "MX4Tensor":
+        """From tensors that are known to fit (the quantisation's own)."""
+        t = cls.__new__(cls)
+        t.codes, t.scales, t.columns = codes, scales, columns
+        return t
+
     @property
     def shape(self) -> torch.Size:
         return torch.Size((self.codes.shape[0], self.columns))
@@ -53,7 +60,22 @@ def quantize(x: torch.Tensor) -> MX4Tensor:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise N.NativeError(f"quantize: rows of at least one element, got shape {tuple(x.shape)}")
     rows = N.as_rows(x.detach())
-    return MX4Tensor(*N.mx4_quantize(rows), rows.shape[1])
+    return MX4Tensor._of(*N.mx4_quantize(rows), rows.shape[1])
+
+
+def _mx4_linear_grads(ctx, dy):
+    rows = N.as_rows(dy)
+    w = ctx.weight
+    dx = db = None
+    if ctx.needs_input_grad[0]:
+        dx = N.mx4_linear_dgrad(rows, w.codes, w.scales, w.columns)
+        dx = dx if dy.dim() == 2 else dx.view(*dy.shape[:-1], w.columns)
+    if ctx.needs_input_grad[1]:
+        db = N.mx4_bias_grad(rows, ctx.bias_dtype)
+    return dx, db, None
+
+
+_mx4_linear_grads_once = once_differentiable(_mx4_linear_grads)
 
 
 class _MX4LinearFn(torch.autograd.Function):
@@ -61,16 +83,13 @@ class _MX4LinearFn(torch.autograd.Function):
     def forward(ctx, x, bias, weight):
         ctx.weight = weight
         ctx.bias_dtype = None if bias is None else bias.dtype
-        return N.mx4_linear(N.as_rows(x), weight.codes, weight.scales, bias).view(*x.shape[:-1], weight.codes.shape[0])
+        y = N.mx4_linear(N.as_rows(x), weight.codes, weight.scales, bias)
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.codes.shape[0])
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        rows = N.as_rows(dy)
-        w = ctx.weight
-        dx = N.mx4_linear_dgrad(rows, w.codes, w.scales, w.columns).view(*dy.shape[:-1], w.columns) if ctx.needs_input_grad[0] else None
-        db = N.mx4_bias_grad(rows, ctx.bias_dtype) if ctx.needs_input_grad[1] else None
-        return dx, db, None
+        # (the wrapper that refuses a second differentiation is only needed where one could follow)
+        return _mx4_linear_grads_once(ctx, dy) if torch.is_grad_enabled() else _mx4_linear_grads(ctx, dy)
 
 
 def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[torch.Tensor] = None,
@@ -92,7 +111,9 @@ def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[
         raise N.NativeError(f"linear: rows {tuple(x.shape)}, weight {tuple(weight.shape)}")
     if out_dtype is not None and out_dtype != x.dtype:
         raise N.NativeError(f"linear: a product with {x.dtype} rows has {x.dtype} results, not {out_dtype}")
-    return _MX4LinearFn.apply(x, None if bias is None else bias.contiguous(), weight)
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    return _MX4LinearFn.apply(x, bias, weight)
 
 
 class MX4Linear(nn.Module):

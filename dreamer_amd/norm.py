@@ -16,25 +16,32 @@ from torch.autograd.function import once_differentiable
 from . import _native as N
 
 
+def _layer_norm_grads(ctx, dy):
+    rows, weight, stats = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dx, dw, db = N.layer_norm_backward(rows, N.as_rows(dy), weight, stats, need[0], need[1], need[2], ctx.bias_dtype)
+    return dx if dx is None or dy.dim() == 2 else dx.view(dy.shape), dw, db, None
+
+
+_layer_norm_grads_once = once_differentiable(_layer_norm_grads)
+
+
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         rows = N.as_rows(x)
-        stats = any(ctx.needs_input_grad[:3])
-        y, mean, rstd = N.layer_norm_forward(rows, weight, bias, eps, stats)
+        need = ctx.needs_input_grad
+        stats = need[0] or need[1] or need[2]
+        y, saved = N.layer_norm_forward(rows, weight, bias, eps, stats)
         if stats:
-            ctx.save_for_backward(rows, weight, mean, rstd)
+            ctx.save_for_backward(rows, weight, saved)
             ctx.bias_dtype = None if bias is None else bias.dtype
-        return y.view(x.shape)
+        return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        rows, weight, mean, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, dw, db = N.layer_norm_backward(rows, N.as_rows(dy), weight, mean, rstd, need[0], weight.dtype if need[1] else None,
-                                           ctx.bias_dtype if need[2] else None)
-        return None if dx is None else dx.view(dy.shape), dw, db, None
+        # (the wrapper that refuses a second differentiation is only needed where one could follow)
+        return _layer_norm_grads_once(ctx, dy) if torch.is_grad_enabled() else _layer_norm_grads(ctx, dy)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -46,7 +53,11 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if x.dim() < 1 or x.shape[-1] < 1:
         raise N.NativeError(f"layer_norm: rows of at least one element, got shape {tuple(x.shape)}")
     if x.is_cuda:
-        return _LayerNormFn.apply(x, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), float(eps))
+        if weight is not None and not weight.is_contiguous():
+            weight = weight.contiguous()
+        if bias is not None and not bias.is_contiguous():
+            bias = bias.contiguous()
+        return _LayerNormFn.apply(x, weight, bias, float(eps))
     N.dtype_id(x, "x")
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and (t.shape != x.shape[-1:] or t.dtype not in (torch.float32, x.dtype) or t.device != x.device):

@@ -569,7 +569,8 @@ int drm_distill_topk_backward(const void* logits, int64_t ld_logits, int32_t dty
  *   linear    : y (M, N) = x W^T + bias with x (M, K) in fp32 / bf16 / fp16 (y the same type; bias any of them or NULL): the products
  *               are exact (x in bf16 parts on the bf16 matrix pipe), sums are fp32.
  *   dgrad     : dx (M, K) = dy W, the input gradient of `linear`.
- *   product   : y (M, N) = X W^T + bias with both operands in 4 bits (scaled matrix instructions), y of y_dtype. */
+ *   product   : y (M, N) = X W^T + bias with both operands in 4 bits (scaled matrix instructions), y of y_dtype.
+ * Products take up to 8388480 rows and reductions of up to 4194304 elements (DRM_ENOTSUP beyond). */
 int drm_mx4_quantize(const void* x, int64_t ldx, int32_t dtype, int64_t rows, int32_t K, uint8_t* codes, uint8_t* scales,
                      drm_stream_t stream);
 int drm_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int32_t K, void* y, int64_t ldy, int32_t dtype,
