@@ -5,6 +5,8 @@
 
 namespace drm {
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 template <typename T>
 struct Elem;
 template <> struct Elem<float> { static constexpr int VEC = 4; static constexpr int ID = DRM_F32; };
@@ -45,6 +47,18 @@ __device__ __forceinline__ void store_slot(T* __restrict__ row, int64_t at, int6
         for (int i = 0; i < VEC; ++i)
             if (at + i < len) row[at + i] = (T)v[i];
     }
+}
+
+// Slot `at` of a row of `len` >= VEC elements without a branch: the slot is moved back into the row where it would leave it, so that
+// every lane's load can be issued before the first one is waited for.  The elements of such a slot that belong to an earlier
+// one (or all of them, behind the row) are not its own: owned(at, len, i) tells.
+template <typename T>
+__device__ __forceinline__ int64_t slot_at(int64_t at, int64_t len) { return at + Elem<T>::VEC <= len ? at : len - Elem<T>::VEC; }
+template <typename T>
+__device__ __forceinline__ bool owned(int64_t at, int64_t len, int i) { return slot_at<T>(at, len) + i >= at; }
+template <typename T>
+__device__ __forceinline__ Slot<T> raw_slot(const T* __restrict__ row, int64_t at, int64_t len) {
+    return *reinterpret_cast<const Slot<T>*>(row + slot_at<T>(at, len));
 }
 
 // a vector of another type held beside the rows (weights, biases): element by runtime type

@@ -4,12 +4,13 @@
 //   dx = r (g - mean(g) - xh mean(g xh)),  g = dy w;      dw = sum over rows of dy xh;      db = sum over rows of dy
 //
 // Both directions are streams: forward reads x and writes y, backward reads x and dy and writes dx.  A row is held in
-// registers between its statistics and its results (one wave for up to 64 x 16 elements, else one workgroup), so that x is
+// registers between its statistics and its results (eight lanes to one wave for up to 64 x 16 elements, else one workgroup), so that x is
 // read once and the variance is taken about the mean.  Workgroups walk over rows: the weight and the bias stay in registers
 // for all of them, and so do the column sums of the backward pass, which go to `partials` once per workgroup and are added
 // there in a fixed order (no atomics: results do not depend on the order in which workgroups run).
 #include "elem.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace drm {
@@ -18,8 +19,9 @@ namespace drm {
 // that one barrier per call is enough.
 template <int TPB>
 __device__ __forceinline__ void row_sum2(float& a, float& b, float (*buf)[2]) {
-    a = group_sum<64>(a);
-    b = group_sum<64>(b);
+    constexpr int G = TPB < 64 ? TPB : 64;
+    a = group_sum<G>(a);
+    b = group_sum<G>(b);
     if constexpr (TPB > 64) {
         constexpr int W = TPB / 64;
         const int w = threadIdx.x >> 6;
@@ -37,196 +39,305 @@ __device__ __forceinline__ float row_sum(float a, float (*buf)[2]) {
     return a;
 }
 
-// TPB threads per row; 64: four rows per workgroup, one per wave
+// What a thread holds of a row: CH slots as they lie in memory, TPB threads per row.  All loads of a row are issued together, and
+// those of the next row before this one is worked on.  Each pass over the part converts anew (`renew` keeps the compiler from
+// holding the fp32 values from one pass to the next: at two bytes an element they would take twice the registers).
 template <typename T, int TPB, int CH>
-__global__ __launch_bounds__(TPB == 64 ? 256 : TPB) void k_norm_fwd(const T* __restrict__ x, int64_t ldx, const void* w, const void* b,
-                                                                    int wtype, T* __restrict__ y, int64_t ldy,
-                                                                    float* __restrict__ mean, float* __restrict__ rstd, int64_t N,
-                                                                    int E, float eps) {
-    constexpr int VEC = Elem<T>::VEC, RPB = TPB == 64 ? 4 : 1;
-    __shared__ float s_buf[2][TPB / 64][2];
-    const int t = TPB == 64 ? (threadIdx.x & 63) : threadIdx.x;
-    float wv[CH][VEC], bv[CH][VEC];
+struct RowPart {
+    static constexpr int VEC = Elem<T>::VEC;
+    Slot<T> s[CH];
+    __device__ __forceinline__ void load(const T* __restrict__ row, int t, int E) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) s[c] = raw_slot(row, (c * TPB + t) * VEC, E);
+    }
+    __device__ __forceinline__ void renew() {
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                u32x4 r = __builtin_bit_cast(u32x4, s[c]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t d = r[k];
+                    asm volatile("" : "+v"(d));
+                    r[k] = d;
+                }
+                s[c] = __builtin_bit_cast(Slot<T>, r);
+            }
+        }
+    }
+    // f(value, c, i) for every element; one that is not its slot's own (see raw_slot) comes as `fill`
+    template <typename F>
+    __device__ __forceinline__ void each(int t, int E, float fill, F&& f) const {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int at = (c * TPB + t) * VEC, foreign = at - (int)slot_at<T>(at, E);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) f(i >= foreign ? (float)s[c].v[i] : fill, c, i);
+        }
+    }
+    // store f(value, c, i); a slot that was moved back writes some of its neighbour's results once more, computed like the others
+    template <typename F>
+    __device__ __forceinline__ void store(T* __restrict__ row, int t, int E, F&& f) const {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int at = (c * TPB + t) * VEC;
+            Slot<T> o;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) o.v[i] = (T)f((float)s[c].v[i], c, i);
+            if (at < E) *reinterpret_cast<Slot<T>*>(row + slot_at<T>(at, E)) = o;
+        }
+    }
+};
+
+// w, b (fp32 or the rows' type) at the positions of a thread's slots; all loads under way together
+template <typename T, int TPB, int CH>
+__device__ __forceinline__ void load_columns(const void* p, int type, float absent, int t, int E, float (&v)[CH][Elem<T>::VEC]) {
+    constexpr int VEC = Elem<T>::VEC;
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int e = (c * TPB + t) * VEC + i;
-            wv[c][i] = w != nullptr && e < E ? load_elem(w, wtype, e) : 1.f;
-            bv[c][i] = b != nullptr && e < E ? load_elem(b, wtype, e) : 0.f;
-        }
-    const float inv = 1.f / (float)E;
-    for (int64_t n = (int64_t)blockIdx.x * RPB + (TPB == 64 ? threadIdx.x >> 6 : 0); n < N; n += (int64_t)gridDim.x * RPB) {
-        const T* row = x + n * ldx;
-        float v[CH][VEC], s = 0.f;
+        for (int i = 0; i < VEC; ++i) v[c][i] = absent;
+    if (p == nullptr) return;
+    if (type == DRM_F32) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            load_slot(row, (int64_t)(c * TPB + t) * VEC, E, 0.f, v[c]);
+            const float* at = reinterpret_cast<const float*>(p) + slot_at<T>((c * TPB + t) * VEC, E);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) s += v[c][i];
-        }
-        const float m = row_sum<TPB>(s, s_buf[0]) * inv;
-        float q = 0.f;
+            for (int h = 0; h < VEC; h += 4) {
+                const Slot<float> s = *reinterpret_cast<const Slot<float>*>(at + h);
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                v[c][i] -= m;
-                if ((c * TPB + t) * VEC + i < E) q += v[c][i] * v[c][i];
+                for (int i = 0; i < 4; ++i) v[c][h + i] = s.v[i];
             }
-        const float r = 1.f / sqrtf(row_sum<TPB>(q, s_buf[1]) * inv + eps);
-        if (t == 0 && mean != nullptr) { mean[n] = m; rstd[n] = r; }
-        T* out = y + n * ldy;
+        }
+    } else {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
+            const Slot<T> s = raw_slot(reinterpret_cast<const T*>(p), (c * TPB + t) * VEC, E);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) v[c][i] = fmaf(v[c][i] * r, wv[c][i], bv[c][i]);
-            store_slot(out, (int64_t)(c * TPB + t) * VEC, E, v[c]);
+            for (int i = 0; i < VEC; ++i) v[c][i] = (float)s.v[i];
         }
     }
 }
 
-// Rows too long for registers: three walks over the row (the second and third find it in the caches unless it is longer than
-// those).  One workgroup per row.
-template <typename T>
-__global__ __launch_bounds__(1024) void k_norm_fwd_long(const T* __restrict__ x, int64_t ldx, const void* w, const void* b, int wtype,
-                                                        T* __restrict__ y, int64_t ldy, float* __restrict__ mean,
-                                                        float* __restrict__ rstd, int64_t N, int E, float eps) {
-    constexpr int VEC = Elem<T>::VEC;
-    __shared__ float s_buf[2][16][2];
+// TPB threads per row: up to 64 one or several rows per wave (256 threads a workgroup), above one workgroup per row.
+// KEEP: the weight and the bias stay in registers from row to row; without, they are read again (rows of more than 16 elements
+// a thread)
+template <typename T, int TPB, int CH, bool KEEP>
+__global__ __launch_bounds__(TPB <= 64 ? 256 : TPB) void k_norm_fwd(const T* __restrict__ x, int64_t ldx, const void* w, const void* b,
+                                                                    int wtype, T* __restrict__ y, int64_t ldy,
+                                                                    float* __restrict__ mean, float* __restrict__ rstd, int64_t N,
+                                                                    int E, float eps) {
+    constexpr int VEC = Elem<T>::VEC, RPB = TPB <= 64 ? 256 / TPB : 1;
+    using Part = RowPart<T, TPB, CH>;
+    __shared__ float s_buf[2][TPB <= 64 ? 1 : TPB / 64][2];
+    const int t = threadIdx.x % TPB;
+    float wv[CH][VEC], bv[CH][VEC];
+    if constexpr (KEEP) {
+        load_columns<T, TPB, CH>(w, wtype, 1.f, t, E, wv);
+        load_columns<T, TPB, CH>(b, wtype, 0.f, t, E, bv);
+    }
     const float inv = 1.f / (float)E;
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    Part next;
+    int64_t n = (int64_t)blockIdx.x * RPB + threadIdx.x / TPB;
+    next.load(x + min(n, N - 1) * ldx, t, E);
+    // (uniform trip count: groups of a workgroup whose rows have run out go on with the last row and store nothing)
+    for (int64_t base = (int64_t)blockIdx.x * RPB; base < N; base += step, n += step) {
+        Part part = next;
+        next.load(x + min(n + step, N - 1) * ldx, t, E);
+        float sum = 0.f, q = 0.f;
+        part.each(t, E, 0.f, [&](float v, int, int) { sum += v; });
+        const float m = row_sum<TPB>(sum, s_buf[0]) * inv;
+        part.renew();
+        part.each(t, E, m, [&](float v, int, int) { q = fmaf(v - m, v - m, q); });
+        const float r = 1.f / sqrtf(row_sum<TPB>(q, s_buf[1]) * inv + eps);
+        if (n >= N) continue;
+        if (t == 0 && mean != nullptr) { mean[n] = m; rstd[n] = r; }
+        if constexpr (!KEEP) {
+            load_columns<T, TPB, CH>(w, wtype, 1.f, t, E, wv);
+            load_columns<T, TPB, CH>(b, wtype, 0.f, t, E, bv);
+        }
+        part.renew();
+        part.store(y + n * ldy, t, E, [&](float v, int c, int i) { return fmaf((v - m) * r, wv[c][i], bv[c][i]); });
+    }
+}
+
+// Rows too long for registers (three walks over the row; the second and third find it in the caches unless it is longer than
+// those) and rows shorter than a slot.  One workgroup per row, four slots under way per thread.
+template <typename T, int TPB>
+__global__ __launch_bounds__(TPB) void k_norm_fwd_long(const T* __restrict__ x, int64_t ldx, const void* w, const void* b, int wtype,
+                                                       T* __restrict__ y, int64_t ldy, float* __restrict__ mean,
+                                                       float* __restrict__ rstd, int64_t N, int E, float eps) {
+    constexpr int VEC = Elem<T>::VEC, U = 4, STEP = TPB * VEC;
+    __shared__ float s_buf[2][TPB / 64][2];
+    const float inv = 1.f / (float)E;
+    const int64_t bulk = (int64_t)E / (U * STEP) * (U * STEP);       // whole slots of every thread
     for (int64_t n = blockIdx.x; n < N; n += gridDim.x) {
         const T* row = x + n * ldx;
-        float v[VEC], s = 0.f, q = 0.f;
-        for (int64_t e = (int64_t)threadIdx.x * VEC; e < E; e += 1024 * VEC) {
-            load_slot(row, e, E, 0.f, v);
+        float s = 0.f, q = 0.f;
+        auto walk = [&](auto&& f) {
+            for (int64_t e = (int64_t)threadIdx.x * VEC; e < bulk; e += U * STEP) {
+                Slot<T> raw[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) raw[u] = *reinterpret_cast<const Slot<T>*>(row + e + u * STEP);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    float v[VEC];
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) v[i] = (float)raw[u].v[i];
+                    f(v, VEC, e + u * STEP);
+                }
+            }
+            for (int64_t e = bulk + (int64_t)threadIdx.x * VEC; e < E; e += STEP) {
+                float v[VEC];
+                load_slot(row, e, E, 0.f, v);
+                f(v, (int)min((int64_t)VEC, E - e), e);
+            }
+        };
+        walk([&](const float (&v)[VEC], int, int64_t) {
             float p = 0.f;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) p += v[i];
             s += p;
-        }
-        const float m = row_sum<1024>(s, s_buf[0]) * inv;
-        for (int64_t e = (int64_t)threadIdx.x * VEC; e < E; e += 1024 * VEC) {
-            load_slot(row, e, E, m, v);
+        });
+        const float m = row_sum<TPB>(s, s_buf[0]) * inv;
+        walk([&](const float (&v)[VEC], int have, int64_t) {
             float p = 0.f;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) p += (v[i] - m) * (v[i] - m);
+            for (int i = 0; i < VEC; ++i) p += i < have ? (v[i] - m) * (v[i] - m) : 0.f;
             q += p;
-        }
-        const float r = 1.f / sqrtf(row_sum<1024>(q, s_buf[1]) * inv + eps);
+        });
+        const float r = 1.f / sqrtf(row_sum<TPB>(q, s_buf[1]) * inv + eps);
         if (threadIdx.x == 0 && mean != nullptr) { mean[n] = m; rstd[n] = r; }
-        for (int64_t e = (int64_t)threadIdx.x * VEC; e < E; e += 1024 * VEC) {
-            load_slot(row, e, E, 0.f, v);
+        walk([&](const float (&v)[VEC], int, int64_t e) {
+            float o[VEC];
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const int64_t k = min(e + i, (int64_t)E - 1);
-                v[i] = fmaf((v[i] - m) * r, w != nullptr ? load_elem(w, wtype, k) : 1.f, b != nullptr ? load_elem(b, wtype, k) : 0.f);
+                o[i] = fmaf((v[i] - m) * r, w != nullptr ? load_elem(w, wtype, k) : 1.f, b != nullptr ? load_elem(b, wtype, k) : 0.f);
             }
-            store_slot(y + n * ldy, e, E, v);
-        }
+            store_slot(y + n * ldy, e, E, o);
+        });
     }
 }
 
 // partials: (gridDim.x, 2, E): column sums of dy xh and of dy over the rows this workgroup walked
 template <typename T, int TPB, int CH>
-__global__ __launch_bounds__(TPB == 64 ? 256 : TPB) void k_norm_bwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy,
+__global__ __launch_bounds__(TPB <= 64 ? 256 : TPB, 4) void k_norm_bwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy,
                                                                     int64_t lddy, const void* w, int wtype,
                                                                     const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                     T* __restrict__ dx, float* __restrict__ partials, int64_t N,
                                                                     int E) {
-    constexpr int VEC = Elem<T>::VEC, RPB = TPB == 64 ? 4 : 1;
-    __shared__ float s_buf[2][TPB / 64][2];
-    __shared__ float s_cols[TPB == 64 ? 64 * CH * VEC : 1];
-    const int t = TPB == 64 ? (threadIdx.x & 63) : threadIdx.x;
+    constexpr int VEC = Elem<T>::VEC, RPB = TPB <= 64 ? 256 / TPB : 1;
+    constexpr bool KEEP = CH * VEC <= 8, AHEAD = KEEP;            // (sixteen elements at 1024 threads: 128 registers each)
+    using Part = RowPart<T, TPB, CH>;
+    __shared__ float s_buf[2][TPB <= 64 ? 1 : TPB / 64][2];
+    __shared__ float s_cols[TPB <= 64 ? TPB * CH * VEC : 1];
+    const int t = threadIdx.x % TPB;
     float wv[CH][VEC], aw[CH][VEC], ab[CH][VEC];
+    if constexpr (KEEP) load_columns<T, TPB, CH>(w, wtype, 1.f, t, E, wv);
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int e = (c * TPB + t) * VEC + i;
-            wv[c][i] = w != nullptr && e < E ? load_elem(w, wtype, e) : 1.f;
-            aw[c][i] = 0.f;
-            ab[c][i] = 0.f;
-        }
+        for (int i = 0; i < VEC; ++i) { aw[c][i] = 0.f; ab[c][i] = 0.f; }
     const float inv = 1.f / (float)E;
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    Part nx, nd;
+    float nm = 0.f, nr = 0.f;
+    int64_t n = (int64_t)blockIdx.x * RPB + threadIdx.x / TPB;
+    auto fetch = [&](int64_t at) {
+        const int64_t k = min(at, N - 1);
+        nx.load(x + k * ldx, t, E);
+        nd.load(dy + k * lddy, t, E);
+        nm = mean[k];
+        nr = rstd[k];
+    };
+    if constexpr (AHEAD) fetch(n);
     int flip = 0;
-    for (int64_t n = (int64_t)blockIdx.x * RPB + (TPB == 64 ? threadIdx.x >> 6 : 0); n < N; n += (int64_t)gridDim.x * RPB, flip ^= 1) {
-        const float m = mean[n], r = rstd[n];
-        float xh[CH][VEC], g[CH][VEC], s = 0.f, q = 0.f;
-#pragma unroll
-        for (int c = 0; c < CH; ++c) load_slot(x + n * ldx, (int64_t)(c * TPB + t) * VEC, E, m, xh[c]);   // beyond the row: xh = 0
-#pragma unroll
-        for (int c = 0; c < CH; ++c) load_slot(dy + n * lddy, (int64_t)(c * TPB + t) * VEC, E, 0.f, g[c]);
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float h = (xh[c][i] - m) * r, d = g[c][i];
-                aw[c][i] = fmaf(d, h, aw[c][i]);
-                ab[c][i] += d;
-                const float gw = d * wv[c][i];
-                s += gw;
-                q = fmaf(gw, h, q);
-                xh[c][i] = h;
-                g[c][i] = gw;
-            }
+    for (int64_t base = (int64_t)blockIdx.x * RPB; base < N; base += step, n += step, flip ^= 1) {
+        if constexpr (!AHEAD) fetch(n);
+        Part px = nx, pd = nd;
+        const float m = nm, r = nr;
+        const bool live = n < N;                                  // (a group of a wave without a row: nothing to add)
+        if constexpr (AHEAD) fetch(n + step);
+        if constexpr (!KEEP) load_columns<T, TPB, CH>(w, wtype, 1.f, t, E, wv);
+        float s = 0.f, q = 0.f;
+        pd.each(t, E, 0.f, [&](float d, int c, int i) {
+            if (TPB <= 64 && !live) d = 0.f;
+            const float h = ((float)px.s[c].v[i] - m) * r, gw = d * wv[c][i];
+            aw[c][i] = fmaf(d, h, aw[c][i]);
+            ab[c][i] += d;
+            s += gw;
+            q = fmaf(gw, h, q);
+        });
         row_sum2<TPB>(s, q, s_buf[flip]);
-        if (dx != nullptr) {
+        if (dx != nullptr && live) {
             s *= inv; q *= inv;
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) g[c][i] = r * (g[c][i] - fmaf(xh[c][i], q, s));
-                store_slot(dx + n * (int64_t)E, (int64_t)(c * TPB + t) * VEC, E, g[c]);
-            }
+            if constexpr (!KEEP) load_columns<T, TPB, CH>(w, wtype, 1.f, t, E, wv);
+            px.renew();
+            pd.renew();
+            pd.store(dx + n * (int64_t)E, t, E, [&](float d, int c, int i) {
+                return r * (fmaf(d, wv[c][i], -s) - ((float)px.s[c].v[i] - m) * r * q);
+            });
         }
     }
     if (partials == nullptr) return;
     float* pw = partials + (int64_t)blockIdx.x * 2 * E;
-    if constexpr (TPB == 64) {   // the four waves' sums, one wave after the other
+    if constexpr (TPB <= 64) {
+        // rows of one wave first, then the four waves one after the other
+        if constexpr (TPB < 64) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    if constexpr (TPB <= 8) { aw[c][i] += xor_lane<8>(aw[c][i]); ab[c][i] += xor_lane<8>(ab[c][i]); }
+                    if constexpr (TPB <= 16) { aw[c][i] += xor_lane<16>(aw[c][i]); ab[c][i] += xor_lane<16>(ab[c][i]); }
+                    aw[c][i] += xor_lane<32>(aw[c][i]); ab[c][i] += xor_lane<32>(ab[c][i]);
+                }
+        }
         const int wave = threadIdx.x >> 6;
+        const bool first = (threadIdx.x & 63) < TPB;
 #pragma unroll
         for (int half = 0; half < 2; ++half)
             for (int k = 0; k < 4; ++k) {
                 __syncthreads();
-                if (wave != k) continue;
+                if (wave != k || !first) continue;
 #pragma unroll
                 for (int c = 0; c < CH; ++c)
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
-                        const int e = (c * TPB + t) * VEC + i;
-                        const float mine = half == 0 ? aw[c][i] : ab[c][i];
-                        const float sum = (k == 0 ? 0.f : s_cols[e]) + mine;
-                        if (k < 3) s_cols[e] = sum;
-                        else if (e < E) pw[(int64_t)half * E + e] = sum;
+                        const int at = (c * TPB + t) * VEC;
+                        const float sum = (k == 0 ? 0.f : s_cols[at + i]) + (half == 0 ? aw[c][i] : ab[c][i]);
+                        if (k < 3) s_cols[at + i] = sum;
+                        else if (at < E && owned<T>(at, E, i)) pw[(int64_t)half * E + slot_at<T>(at, E) + i] = sum;
                     }
             }
     } else {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
+        for (int c = 0; c < CH; ++c)
 #pragma unroll
-            for (int h = 0; h < VEC; h += 4) {
-                const float a[4] = {aw[c][h], aw[c][h + 1], aw[c][h + 2], aw[c][h + 3]};
-                const float b[4] = {ab[c][h], ab[c][h + 1], ab[c][h + 2], ab[c][h + 3]};
-                store_slot(pw, (int64_t)(c * TPB + t) * VEC + h, E, a);
-                store_slot(pw + E, (int64_t)(c * TPB + t) * VEC + h, E, b);
+            for (int i = 0; i < VEC; ++i) {
+                const int at = (c * TPB + t) * VEC;
+                if (at < E && owned<T>(at, E, i)) {
+                    pw[slot_at<T>(at, E) + i] = aw[c][i];
+                    pw[E + slot_at<T>(at, E) + i] = ab[c][i];
+                }
             }
-        }
     }
 }
 
-// rows too long for registers: the two row means first ...
-template <typename T>
-__global__ __launch_bounds__(1024) void k_norm_bwd_sums(const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy, int64_t lddy,
+// the same rows backward: the two row means first ...
+template <typename T, int TPB>
+__global__ __launch_bounds__(TPB) void k_norm_bwd_sums(const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy, int64_t lddy,
                                                         const void* w, int wtype, const float* __restrict__ mean,
                                                         const float* __restrict__ rstd, float* __restrict__ sums, int64_t N, int E) {
     constexpr int VEC = Elem<T>::VEC;
-    __shared__ float s_buf[2][16][2];
+    __shared__ float s_buf[2][TPB / 64][2];
     int flip = 0;
     for (int64_t n = blockIdx.x; n < N; n += gridDim.x, flip ^= 1) {
         const float m = mean[n], r = rstd[n];
         float xv[VEC], g[VEC], s = 0.f, q = 0.f;
-        for (int64_t e = (int64_t)threadIdx.x * VEC; e < E; e += 1024 * VEC) {
+        for (int64_t e = (int64_t)threadIdx.x * VEC; e < E; e += TPB * VEC) {
             load_slot(x + n * ldx, e, E, m, xv);
             load_slot(dy + n * lddy, e, E, 0.f, g);
             float ps = 0.f, pq = 0.f;
@@ -238,7 +349,7 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_sums(const T* __restrict__ x,
             }
             s += ps; q += pq;
         }
-        row_sum2<1024>(s, q, s_buf[flip]);
+        row_sum2<TPB>(s, q, s_buf[flip]);
         if (threadIdx.x == 0) { sums[2 * n] = s / (float)E; sums[2 * n + 1] = q / (float)E; }
     }
 }
@@ -281,57 +392,77 @@ __global__ __launch_bounds__(256) void k_norm_bwd_cols(const T* __restrict__ x, 
     }
 }
 
-// Column sums over the slices: 64 columns x 4 slice groups per workgroup, groups added in order.  Column c < E: dw, else db.
-__global__ __launch_bounds__(256) void k_norm_cols(const float* __restrict__ partials, int slices, int E, int wtype, void* dw, void* db) {
-    __shared__ float s_part[4][64];
-    const int g = threadIdx.x >> 6, l = threadIdx.x & 63;
-    const int64_t c = (int64_t)blockIdx.x * 64 + l, cols = 2 * (int64_t)E;
-    float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+// Column sums over the slices: 32 columns x 32 groups of slices per workgroup (the sum is short of bytes and long of latency: eight
+// loads under way per thread), groups added in order.  Column c < E: dw, else db.
+__global__ __launch_bounds__(1024) void k_norm_cols(const float* __restrict__ partials, int slices, int E, int wtype, void* dw, void* db) {
+    __shared__ float s_part[32][33];
+    const int g = threadIdx.x >> 5, l = threadIdx.x & 31;
+    const int64_t c = (int64_t)blockIdx.x * 32 + l, cols = 2 * (int64_t)E;
+    float a[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) a[u] = 0.f;
     if (c < cols) {
         int s = g;
-        for (; s + 12 < slices; s += 16) {
-            a0 += partials[(int64_t)s * cols + c];
-            a1 += partials[(int64_t)(s + 4) * cols + c];
-            a2 += partials[(int64_t)(s + 8) * cols + c];
-            a3 += partials[(int64_t)(s + 12) * cols + c];
+        for (; s + 7 * 32 < slices; s += 8 * 32) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = partials[(int64_t)(s + u * 32) * cols + c];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) a[u] += v[u];
         }
-        for (; s < slices; s += 4) a0 += partials[(int64_t)s * cols + c];
+        for (; s < slices; s += 32) a[0] += partials[(int64_t)s * cols + c];
     }
-    s_part[g][l] = (a0 + a1) + (a2 + a3);
+    s_part[g][l] = ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
     __syncthreads();
     if (g == 0 && c < cols) {
-        const float v = (s_part[0][l] + s_part[1][l]) + (s_part[2][l] + s_part[3][l]);
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v += s_part[k][l];
         if (c < E) { if (dw != nullptr) store_elem(dw, wtype, c, v); }
         else if (db != nullptr) store_elem(db, wtype, c - E, v);
     }
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------
-// Threads per row by the row's length: enough for 16 elements a thread (16 values, weights and two running column sums fit
-// the registers at four waves per SIMD).
-constexpr int NORM_MAX_E = 1024 * 16;
-static inline int norm_threads(int E) { return E <= 1024 ? 64 : E <= 4096 ? 256 : E <= 8192 ? 512 : 1024; }
-// workgroups that walk the rows
-static inline int norm_slices(int64_t N, int E) {
-    if (E > NORM_MAX_E) return (int)(N < 64 ? (N > 0 ? N : 1) : 64);
-    const int tpb = norm_threads(E);
-    const int64_t rows = tpb == 64 ? (N + 3) / 4 : N, cap = 512;
-    return (int)(rows < 1 ? 1 : rows < cap ? rows : cap);
+// Threads per row by the row's length.  Backward holds eight elements a thread (x, dy, the next row's, weight, two running column
+// sums: 80 to 100 registers, four to five waves per SIMD) up to 8192, sixteen at 1024 threads; forward sixteen, 32 at 1024 threads.
+constexpr int NORM_MAX_E = 1024 * 16, NORM_MAX_E_FWD = 1024 * 32;
+template <typename T>
+static inline bool norm_short(int E) { return E < Elem<T>::VEC; }
+static inline bool norm_long_bwd(int E, int x_dtype) { return E > NORM_MAX_E || E < (x_dtype == DRM_F32 ? 4 : 8); }
+// workgroups that walk the rows backward (about sixteen waves a CU): each leaves 2 E column sums
+static inline int norm_slices(int64_t N, int E, int x_dtype) {
+    if (N < 1) return 1;
+    if (norm_long_bwd(E, x_dtype)) return (int)(N < 64 ? N : 64);
+    const int vec = x_dtype == DRM_F32 ? 4 : 8;
+    const int64_t rpb = E <= 8 * vec ? 32 : E <= 16 * vec ? 16 : E <= 32 * vec ? 8 : E <= 512 ? 4 : 1, groups = (N + rpb - 1) / rpb;
+    const int64_t cap = E <= 512 ? 1024 : E <= 1024 ? 2048 : E <= 2048 ? 1024 : E <= 4096 ? 512 : 256;
+    return (int)(groups < cap ? groups : cap);
 }
 
-template <typename T, typename F>
+#define DRM_NORM_CASE(TPB, CH) return f(std::integral_constant<int, TPB>{}, std::integral_constant<int, CH>{})
+template <typename T, bool BWD, typename F>
 static int norm_variant(int E, F&& f) {
     constexpr int VEC = Elem<T>::VEC, C8 = 8 / VEC, C16 = 16 / VEC;
-#define DRM_NORM_CASE(TPB, CH) return f(std::integral_constant<int, TPB>{}, std::integral_constant<int, CH>{})
+    if (E <= 8 * VEC) DRM_NORM_CASE(8, 1);
+    if (E <= 16 * VEC) DRM_NORM_CASE(16, 1);
+    if (E <= 32 * VEC) DRM_NORM_CASE(32, 1);
     if (E <= 64 * VEC) DRM_NORM_CASE(64, 1);
     if (E <= 512) DRM_NORM_CASE(64, C8);
-    if (E <= 1024) DRM_NORM_CASE(64, C16);
-    if (E <= 2048) DRM_NORM_CASE(256, C8);
-    if (E <= 4096) DRM_NORM_CASE(256, C16);
-    if (E <= 8192) DRM_NORM_CASE(512, C16);
+    if constexpr (BWD) {
+        if (E <= 1024) DRM_NORM_CASE(128, C8);
+        if (E <= 2048) DRM_NORM_CASE(256, C8);
+        if (E <= 4096) DRM_NORM_CASE(512, C8);
+        if (E <= 8192) DRM_NORM_CASE(1024, C8);
+    } else {
+        if (E <= 1024) DRM_NORM_CASE(64, C16);
+        if (E <= 2048) DRM_NORM_CASE(256, C8);
+        if (E <= 4096) DRM_NORM_CASE(256, C16);
+        if (E <= 8192) DRM_NORM_CASE(512, C16);
+    }
     DRM_NORM_CASE(1024, C16);
-#undef DRM_NORM_CASE
 }
+#undef DRM_NORM_CASE
 
 static int norm_check(const char* what, const void* x, int64_t ldx, int x_dtype, int w_dtype, int64_t N, int32_t E) {
     DRM_REQUIRE(x, DRM_EINVAL, "%s: null pointer", what);
@@ -357,14 +488,18 @@ extern "C" int drm_layer_norm_forward(const void* x, int64_t ldx, int32_t x_dtyp
     ProfScope ps(PC_ELEMENTWISE, s, 8 * n, 2 * n * elem_bytes(x_dtype));
     return with_elem(x_dtype, [&](auto tag) -> int {
         using T = decltype(tag);
-        if (E > NORM_MAX_E) {
-            k_norm_fwd_long<T><<<(int)(N < 2048 ? N : 2048), 1024, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
+        const int long_grid = (int)(N < 4096 ? N : 4096);
+        if (norm_short<T>(E)) {
+            k_norm_fwd_long<T, 64><<<long_grid, 64, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
+        } else if (E > NORM_MAX_E_FWD) {
+            k_norm_fwd_long<T, 1024><<<long_grid, 1024, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
+        } else if (E > NORM_MAX_E) {
+            k_norm_fwd<T, 1024, 32 / Elem<T>::VEC, false><<<(int)(N < 512 ? N : 512), 1024, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
         } else {
-            norm_variant<T>(E, [&](auto tpb, auto ch) {
-                constexpr int TPB = decltype(tpb)::value, CH = decltype(ch)::value;
-                const int64_t rows = TPB == 64 ? (N + 3) / 4 : N;
-                const int grid = (int)(rows < 2048 ? rows : 2048);
-                k_norm_fwd<T, TPB, CH><<<grid, TPB == 64 ? 256 : TPB, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
+            norm_variant<T, false>(E, [&](auto tpb, auto ch) {
+                constexpr int TPB = decltype(tpb)::value, CH = decltype(ch)::value, RPB = TPB <= 64 ? 256 / TPB : 1;
+                const int64_t groups = (N + RPB - 1) / RPB, cap = 256 * 2048 / (TPB <= 64 ? 256 : TPB);   // what the chip holds at once
+                k_norm_fwd<T, TPB, CH, true><<<(int)(groups < cap ? groups : cap), TPB <= 64 ? 256 : TPB, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
                 return 0;
             });
         }
@@ -373,10 +508,15 @@ extern "C" int drm_layer_norm_forward(const void* x, int64_t ldx, int32_t x_dtyp
     });
 }
 
+// (the larger of what the row types need)
 extern "C" size_t drm_layer_norm_workspace_bytes(int64_t N, int32_t E) {
     if (N < 0 || E < 1) return 0;
-    const size_t sums = E > NORM_MAX_E ? (size_t)N * 2 * sizeof(float) : 0;
-    return sums + (size_t)norm_slices(N, E) * 2 * E * sizeof(float);
+    size_t need = 0;
+    for (int t : {DRM_F32, DRM_BF16}) {
+        const size_t sums = norm_long_bwd(E, t) ? (size_t)N * 2 * sizeof(float) : 0;
+        need = std::max(need, sums + (size_t)norm_slices(N, E, t) * 2 * E * sizeof(float));
+    }
+    return need;
 }
 
 extern "C" int drm_layer_norm_backward(const void* x, int64_t ldx, const void* dy, int64_t lddy, int32_t x_dtype, const void* w,
@@ -386,9 +526,9 @@ extern "C" int drm_layer_norm_backward(const void* x, int64_t ldx, const void* d
     const bool cols = dw != nullptr || db != nullptr;
     DRM_REQUIRE(N >= 0 && E >= 1, DRM_EINVAL, "N=%lld E=%d", (long long)N, E);
     DRM_REQUIRE(elem_ok(x_dtype) && (w_dtype == DRM_F32 || w_dtype == x_dtype), DRM_ENOTSUP, "element types %d / %d", x_dtype, w_dtype);
-    const int cgrid = (int)((2 * (int64_t)E + 63) / 64);
+    const int cgrid = (int)((2 * (int64_t)E + 31) / 32);
     if (N == 0) {
-        if (cols) { k_norm_cols<<<cgrid, 256, 0, s>>>(nullptr, 0, E, w_dtype, dw, db); DRM_LAUNCH_CHECK(); }
+        if (cols) { k_norm_cols<<<cgrid, 1024, 0, s>>>(nullptr, 0, E, w_dtype, dw, db); DRM_LAUNCH_CHECK(); }
         return DRM_OK;
     }
     if (int rc = norm_check(__func__, x, ldx, x_dtype, w_dtype, N, E)) return rc;
@@ -396,25 +536,28 @@ extern "C" int drm_layer_norm_backward(const void* x, int64_t ldx, const void* d
     if (!dx && !cols) return DRM_OK;
     DRM_REQUIRE(workspace && workspace_bytes >= drm_layer_norm_workspace_bytes(N, E), DRM_EINVAL, "workspace of %zu bytes, %zu needed",
                 workspace ? workspace_bytes : (size_t)0, drm_layer_norm_workspace_bytes(N, E));
-    const int slices = norm_slices(N, E);
+    const int slices = norm_slices(N, E, x_dtype);
+    const bool walk = norm_long_bwd(E, x_dtype);
     const double n = (double)N * E;
     ProfScope ps(PC_ELEMENTWISE, s, 17 * n, 3 * n * elem_bytes(x_dtype));
     float* sums = (float*)workspace;
-    float* part = !cols ? nullptr : E > NORM_MAX_E ? sums + 2 * N : sums;
+    float* part = !cols ? nullptr : walk ? sums + 2 * N : sums;
     const int rc = with_elem(x_dtype, [&](auto tag) -> int {
         using T = decltype(tag);
-        if (E > NORM_MAX_E) {
+        if (walk) {
             if (dx != nullptr) {
-                k_norm_bwd_sums<T><<<(int)(N < 2048 ? N : 2048), 1024, 0, s>>>((const T*)x, ldx, (const T*)dy, lddy, w, w_dtype, mean, rstd, sums, N, E);
+                const int grid = (int)(N < 4096 ? N : 4096);
+                if (norm_short<T>(E)) k_norm_bwd_sums<T, 64><<<grid, 64, 0, s>>>((const T*)x, ldx, (const T*)dy, lddy, w, w_dtype, mean, rstd, sums, N, E);
+                else k_norm_bwd_sums<T, 1024><<<grid, 1024, 0, s>>>((const T*)x, ldx, (const T*)dy, lddy, w, w_dtype, mean, rstd, sums, N, E);
                 DRM_LAUNCH_CHECK();
             }
             constexpr int STRIP = 256 * Elem<T>::VEC;
             k_norm_bwd_cols<T><<<dim3((unsigned)(((int64_t)E + STRIP - 1) / STRIP), slices), 256, 0, s>>>((const T*)x, ldx, (const T*)dy, lddy, w, w_dtype, mean, rstd,
                                                                                       dx != nullptr ? sums : nullptr, (T*)dx, part, N, E);
         } else {
-            norm_variant<T>(E, [&](auto tpb, auto ch) {
+            norm_variant<T, true>(E, [&](auto tpb, auto ch) {
                 constexpr int TPB = decltype(tpb)::value, CH = decltype(ch)::value;
-                k_norm_bwd<T, TPB, CH><<<slices, TPB == 64 ? 256 : TPB, 0, s>>>((const T*)x, ldx, (const T*)dy, lddy, w, w_dtype, mean, rstd, (T*)dx, part, N, E);
+                k_norm_bwd<T, TPB, CH><<<slices, TPB <= 64 ? 256 : TPB, 0, s>>>((const T*)x, ldx, (const T*)dy, lddy, w, w_dtype, mean, rstd, (T*)dx, part, N, E);
                 return 0;
             });
         }
@@ -422,7 +565,7 @@ extern "C" int drm_layer_norm_backward(const void* x, int64_t ldx, const void* d
         return DRM_OK;
     });
     if (rc != DRM_OK || !cols) return rc;
-    k_norm_cols<<<cgrid, 256, 0, s>>>(part, slices, E, w_dtype, dw, db);
+    k_norm_cols<<<cgrid, 1024, 0, s>>>(part, slices, E, w_dtype, dw, db);
     DRM_LAUNCH_CHECK();
     return DRM_OK;
 }
