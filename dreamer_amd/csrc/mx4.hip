@@ -91,60 +91,181 @@ __device__ __forceinline__ void mx4_tile_of(int id, int tiles_m, int tiles_n, in
     tn = (pos - g * group) / rows;
 }
 
+// what lies behind the last block of a row: sixteen zero bytes in memory
+__device__ const uint4 mx4_zero_block = {0u, 0u, 0u, 0u};
+
 // ---- y = x W^T + bias, few rows -----------------------------------------------------------------------------------------
-// The weight is streamed once: a workgroup takes 16 weight rows, its waves split the blocks.  A lane holds one block of one
-// weight row (16 bytes, one scale) and feeds it to four matrix instructions, eight elements each; the four lane groups of an
-// instruction hold four different blocks, which is a permutation of the reduction index that the x operand follows.
-template <typename T, int MT, int NW>
+// The weight is streamed once.  A workgroup takes 16 NT weight rows, its NW waves share the reduction in passes of four blocks (128
+// elements).  In the matrix instruction lanes 0-15 are sixteen rows, so fragments read straight from memory would touch a cache
+// line per lane, and the address path, at a line a clock, would take three times the time of the bytes.  Each wave therefore
+// brings its pass to LDS of its own by direct loads (16 weight rows of 64 bytes, MT x 16 rows of x), two passes under way, and
+// reads the fragments there.  A lane holds one block of a weight row and feeds it to four instructions, eight elements at a
+// time; the four lane groups hold different blocks, a permutation of the reduction index that x follows.  x comes from L2 for every
+// workgroup, which is why a wave takes NT weight tiles to one fragment of x.  The waves' sums meet in LDS in a fixed order.
+template <typename T, int MT, int NT, int NW>
+struct RowsStage {
+    __attribute__((aligned(16))) uint8_t w[NW][NT * 1024], x[NW][MT * 16 * 128 * sizeof(T)];
+    uint32_t sc[NW][NT * 64];
+};
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {        // no more than N vector memory operations under way, LDS reads done
+    static_assert(N < 64);
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0070);
+    asm volatile("" ::: "memory");
+}
+
+template <typename T, int MT, int NT, int NW>
+__device__ __forceinline__ void mx4_rows_store(f32x4* s_acc, const f32x4 (&acc)[NT][MT], const Mx4& W, const void* bias, int btype,
+                                               T* __restrict__ y, int64_t ldy, int M, int n0) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) s_acc[((w * NT + i) * MT + t) * 64 + lane] = acc[i][t];
+    __syncthreads();
+    for (int o = threadIdx.x; o < NT * MT * 64; o += NW * 64) {
+        const int i = o / (MT * 64), t = (o >> 6) % MT, l = o & 63;
+        f32x4 v = s_acc[o];
+#pragma unroll
+        for (int k = 1; k < NW; ++k) v += s_acc[k * NT * MT * 64 + o];
+        const int m = t * 16 + (l & 15), nn = n0 + i * 16 + 4 * (l >> 4);
+        if (m < M)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (nn + e < W.rows) y[m * ldy + nn + e] = (T)(v[e] + (bias != nullptr ? load_elem(bias, btype, nn + e) : 0.f));
+    }
+}
+
+template <typename T, int MT, int NT, int NW>
 __global__ __launch_bounds__(NW * 64) void k_mx4_rows(const T* __restrict__ x, int64_t ldx, Mx4 W, const void* bias, int btype,
                                                       T* __restrict__ y, int64_t ldy, int M, int K) {
-    constexpr int P = Parts<T>::N;
-    __shared__ f32x4 s_acc[NW][MT][64];
+    constexpr int P = Parts<T>::N, EPC = 16 / sizeof(T), XCH = 128 / EPC, XI = MT * 16 * XCH / 64, LOADS = 2 * NT + XI;
+    using Stage = RowsStage<T, MT, NT, NW>;
+    __shared__ Stage s0, s1;
+    static_assert(sizeof(Stage) >= NW * NT * MT * 64 * sizeof(f32x4), "the waves' sums fit one stage");
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-    const int n0 = blockIdx.x * 16;
-    const int64_t n = min(n0 + c, W.rows - 1);
-    f32x4 acc[MT];
+    const int n0 = blockIdx.x * 16 * NT;
+    f32x4 acc[NT][MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int base = w * 4; base < W.nb; base += NW * 4) {
-        const int kb = base + g;
-        const bool live = kb < W.nb;
-        u32x4 q{0, 0, 0, 0};
-        float sc = 1.f;
-        if (live) {
-            q = *reinterpret_cast<const u32x4*>(W.codes + (n * W.nb + kb) * 16);
-            sc = mx4_scale(W.scales[n * W.nb + kb]);
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int turns = ((W.nb + 3) / 4 + NW - 1) / NW;          // this wave's passes: w, w + NW, ...; behind the last block: zero blocks
+    auto issue = [&](Stage& st, int i) {
+        asm volatile("" ::: "memory");
+        const int base = (w + i * NW) * 4;
+        // a lane's own scale byte of each weight tile, widened to a dword by the load
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const uint8_t* src = W.scales + (int64_t)min(n0 + t * 16 + c, W.rows - 1) * W.nb + min(base + g, W.nb - 1);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src,
+                                             (__attribute__((address_space(3))) uint32_t*)(st.sc[w] + t * 64), 1, 0, 0);
+        }
+        // slot p of weight row r holds block p ^ (r / 4): sixteen rows of one block lie on different banks
+        const int wr = lane >> 2, kb = base + ((lane & 3) ^ ((wr >> 2) & 3));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const uint8_t* src = W.codes + ((int64_t)min(n0 + t * 16 + wr, W.rows - 1) * W.nb + kb) * 16;
+            src = kb < W.nb ? src : reinterpret_cast<const uint8_t*>(&mx4_zero_block);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src,
+                                             (__attribute__((address_space(3))) uint32_t*)(st.w[w] + t * 1024), 16, 0, 0);
         }
 #pragma unroll
+        for (int j = 0; j < XI; ++j) {
+            const int slot = j * 64 + lane, r = slot / XCH, p = slot % XCH, k = base * 32 + ((p & 16) | ((p ^ r) & 15)) * EPC;
+            const uint8_t* src = reinterpret_cast<const uint8_t*>(x + (int64_t)min(r, M - 1) * ldx + k);
+            src = k < K ? src : reinterpret_cast<const uint8_t*>(&mx4_zero_block);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src,
+                                             (__attribute__((address_space(3))) uint32_t*)(st.x[w] + j * 1024), 16, 0, 0);
+        }
+        asm volatile("" ::: "memory");
+    };
+    auto compute = [&](const Stage& st) {
+        u32x4 q[NT];
+        float sc[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) sc[i] = mx4_scale(st.sc[w][i * 64 + lane]);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) q[i] = *reinterpret_cast<const u32x4*>(st.w[w] + i * 1024 + c * 64 + ((g ^ ((c >> 2) & 3)) * 16));
+#pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const bf16x8 a = mx4_bf16x8(q[s], sc);
+            bf16x8 a[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) a[i] = mx4_bf16x8(q[i][s], sc[i]);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                Eight<T> e;
+#pragma unroll
+                for (int h = 0; h < 8 / EPC; ++h) {
+                    const int ch = (g * 32 + s * 8) / EPC + h;
+                    reinterpret_cast<u32x4*>(&e)[h] = *reinterpret_cast<const u32x4*>(st.x[w] + ((t * 16 + c) * XCH + ((ch & 16) | ((ch ^ c) & 15))) * 16);
+                }
+                bf16x8 b[P];
+                split_eight<T>(e, b);
+#pragma unroll
+                for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[p], acc[i][t], 0, 0, 0);
+            }
+        }
+    };
+    issue(s0, 0);
+    if (turns == 1) {
+        wait_loads<0>();
+        compute(s0);
+    } else {
+        issue(s1, 1);
+        for (int i = 0; i + 2 < turns; i += 2) {
+            wait_loads<LOADS>();              // the other stage's loads may still be under way
+            compute(s0);
+            wait_loads<63>();
+            issue(s0, i + 2);
+            wait_loads<LOADS>();
+            compute(s1);
+            wait_loads<63>();
+            issue(s1, i + 3);
+        }
+        wait_loads<LOADS>();
+        compute(s0);
+        wait_loads<0>();
+        compute(s1);
+    }
+    __syncthreads();
+    mx4_rows_store<T, MT, NT, NW>(reinterpret_cast<f32x4*>(&s0), acc, W, bias, btype, y, ldy, M, n0);
+}
+
+// The same product for rows of x that direct loads cannot take (not aligned to 16 bytes, or not whole chunks): fragments from memory.
+template <typename T, int MT, int NW>
+__global__ __launch_bounds__(NW * 64) void k_mx4_rows_any(const T* __restrict__ x, int64_t ldx, Mx4 W, const void* bias, int btype,
+                                                          T* __restrict__ y, int64_t ldy, int M, int K) {
+    constexpr int P = Parts<T>::N;
+    __shared__ f32x4 s_acc[NW * MT * 64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int n0 = blockIdx.x * 16;
+    const int64_t row = (int64_t)min(n0 + c, W.rows - 1) * W.nb;
+    f32x4 acc[1][MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[0][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int base = w * 4; base < W.nb; base += NW * 4) {
+        const int kb = base + g;
+        const bool live = kb < W.nb;                     // a block behind the last one: zero codes at scale 1
+        const u32x4 q = reinterpret_cast<const u32x4*>(W.codes)[row + min(kb, W.nb - 1)];
+        const float sc = mx4_scale(live ? W.scales[row + min(kb, W.nb - 1)] : 127u);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const bf16x8 a = mx4_bf16x8(live ? q[s] : 0u, sc);
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 bf16x8 b[P];
                 load_parts(x + (int64_t)min(t * 16 + c, M - 1) * ldx, (int64_t)kb * 32 + s * 8, K, b);
 #pragma unroll
-                for (int p = P - 1; p >= 0; --p) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[p], acc[t], 0, 0, 0);
+                for (int p = P - 1; p >= 0; --p) acc[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[p], acc[0][t], 0, 0, 0);
             }
         }
     }
-#pragma unroll
-    for (int t = 0; t < MT; ++t) s_acc[w][t][lane] = acc[t];
-    __syncthreads();
-    for (int o = threadIdx.x; o < MT * 64; o += NW * 64) {
-        const int t = o >> 6, l = o & 63;
-        f32x4 v = s_acc[0][t][l];
-#pragma unroll
-        for (int k = 1; k < NW; ++k) v += s_acc[k][t][l];
-        const int m = t * 16 + (l & 15), nn = n0 + 4 * (l >> 4);
-        if (m < M)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (nn + i < W.rows) y[m * ldy + nn + i] = (T)(v[i] + (bias != nullptr ? load_elem(bias, btype, nn + i) : 0.f));
-    }
+    mx4_rows_store<T, MT, 1, NW>(s_acc, acc, W, bias, btype, y, ldy, M, n0);
 }
-
-// what lies behind the last block of a row: sixteen zero bytes in memory
-__device__ const uint4 mx4_zero_block = {0u, 0u, 0u, 0u};
 
 // A row's NB blocks of a step in LDS: block b in slot b ^ (the row's number), so that eight rows of one block fall on all banks
 template <int NB>
@@ -697,6 +818,32 @@ static void mx4_launch_tile(const T* x, int64_t ldx, const Mx4& W, const void* b
     }
     k_mx4_tile<T, Parts<T>::N == 1 ? 128 : 64, false, GRAD, false><<<tm * tn, TILE_THREADS, 0, s>>>(x, ldx, W, bias, btype, y, ldy, M, N, K, tm, tn);
 }
+// Few rows: as many weight tiles per wave as leave about one workgroup a CU (x is read once per workgroup); eight waves where two
+// stages of their passes fit the LDS, else four.
+constexpr int MX4_FEW_ROWS = 32;
+template <typename T, int MT>
+static void mx4_launch_rows_mt(const T* x, int64_t ldx, const Mx4& W, const void* bias, int btype, T* y, int64_t ldy, int M, int N, int K, hipStream_t s) {
+    constexpr int EPC = 16 / sizeof(T), NW = MT * sizeof(T) <= 2 ? 8 : 4, MAX_NT = MT * sizeof(T) <= 4 ? 4 : 2;
+    if (!aligned16(x) || ldx % EPC != 0 || K % 8 != 0) {
+        k_mx4_rows_any<T, MT, 8><<<(N + 15) / 16, 512, 0, s>>>(x, ldx, W, bias, btype, y, ldy, M, K);
+        return;
+    }
+    auto go = [&](auto nt) {
+        constexpr int NT = decltype(nt)::value;
+        k_mx4_rows<T, MT, NT, NW><<<(N + 16 * NT - 1) / (16 * NT), NW * 64, 0, s>>>(x, ldx, W, bias, btype, y, ldy, M, K);
+    };
+    if constexpr (MAX_NT == 4) {
+        if (N >= 64 * 192) { go(std::integral_constant<int, 4>{}); return; }
+    }
+    if (N >= 32 * 192) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 1>{});
+}
+template <typename T>
+static void mx4_launch_rows(const T* x, int64_t ldx, const Mx4& W, const void* bias, int btype, T* y, int64_t ldy, int M, int N, int K, hipStream_t s) {
+    if (M <= 16) mx4_launch_rows_mt<T, 1>(x, ldx, W, bias, btype, y, ldy, M, N, K, s);
+    else mx4_launch_rows_mt<T, 2>(x, ldx, W, bias, btype, y, ldy, M, N, K, s);
+}
+
 static int mx4_check_tiles(const char* what, int M, int N, int K) {
     DRM_REQUIRE(K <= (1 << 22), DRM_ENOTSUP, "%s: a row of %d elements (at most 4194304)", what, K);
     DRM_REQUIRE(M <= 65535 * 128, DRM_ENOTSUP, "%s: M=%d rows (at most %d)", what, M, 65535 * 128);
@@ -751,13 +898,10 @@ extern "C" int drm_mx4_linear(const void* x, int64_t ldx, int32_t dtype, const u
     if (int rc = mx4_check_tiles(__func__, M, N, K)) return rc;
     hipStream_t s = (hipStream_t)stream;
     const Mx4 W{codes, scales, N, mx4_blocks(K)};
-    ProfScope ps(M <= 64 ? PC_LINEAR : PC_LINEAR_BIG, s, 2.0 * M * N * K, ((double)M * K + (double)M * N) * elem_bytes(dtype) + (double)N * W.nb * 17);
+    ProfScope ps(M <= MX4_FEW_ROWS ? PC_LINEAR : PC_LINEAR_BIG, s, 2.0 * M * N * K, ((double)M * K + (double)M * N) * elem_bytes(dtype) + (double)N * W.nb * 17);
     return with_elem(dtype, [&](auto tag) -> int {
         using T = decltype(tag);
-        const int grid = (N + 15) / 16;
-        if (M <= 16) k_mx4_rows<T, 1, 8><<<grid, 512, 0, s>>>((const T*)x, ldx, W, bias, bias_dtype, (T*)y, ldy, M, K);
-        else if (M <= 32) k_mx4_rows<T, 2, 8><<<grid, 512, 0, s>>>((const T*)x, ldx, W, bias, bias_dtype, (T*)y, ldy, M, K);
-        else if (M <= 64) k_mx4_rows<T, 4, 8><<<grid, 512, 0, s>>>((const T*)x, ldx, W, bias, bias_dtype, (T*)y, ldy, M, K);
+        if (M <= MX4_FEW_ROWS) mx4_launch_rows<T>((const T*)x, ldx, W, bias, bias_dtype, (T*)y, ldy, M, N, K, s);
         else mx4_launch_tile<false, T>((const T*)x, ldx, W, bias, bias_dtype, (T*)y, ldy, M, N, K, s);
         DRM_LAUNCH_CHECK();
         return DRM_OK;
