@@ -178,14 +178,17 @@ SIGNATURES = {
                                             C.c_int64, C.c_int32, C.c_int32, C.c_double, C.c_void_p, C.c_void_p]),
     "drm_mx4_quantize": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]),
     "drm_mx4_dequantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p]),
+    "drm_mx4_linear_workspace_bytes": (C.c_size_t, [C.c_int32] * 4),
     "drm_mx4_linear": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64]
-                       + [C.c_int32] * 3 + [C.c_void_p]),
+                       + [C.c_int32] * 3 + [C.c_void_p, C.c_size_t, C.c_void_p]),
+    "drm_mx4_linear_dgrad_workspace_bytes": (C.c_size_t, [C.c_int32] * 4),
     "drm_mx4_linear_dgrad": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64] + [C.c_int32] * 3
-                             + [C.c_void_p]),
+                             + [C.c_void_p, C.c_size_t, C.c_void_p]),
     "drm_mx4_bias_grad_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32]),
     "drm_mx4_bias_grad": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_size_t,
                                     C.c_void_p]),
-    "drm_mx4_product": (C.c_int, [C.c_void_p] * 5 + [C.c_int32, C.c_void_p, C.c_int64] + [C.c_int32] * 4 + [C.c_void_p]),
+    "drm_mx4_product_workspace_bytes": (C.c_size_t, [C.c_int32] * 3),
+    "drm_mx4_product": (C.c_int, [C.c_void_p] * 5 + [C.c_int32, C.c_void_p, C.c_int64] + [C.c_int32] * 4 + [C.c_void_p, C.c_size_t, C.c_void_p]),
 }
 
 
@@ -944,8 +947,9 @@ def mx4_linear(x, codes, scales, bias=None) -> torch.Tensor:
     bid = _mx4_bias(bias, N, device, "mx4_linear")
     y = torch.empty((M, N), dtype=x.dtype, device=x.device)
     if M and N:
+        ws, need = _workspace(x.device, "drm_mx4_linear_workspace_bytes", xid, M, N, K)
         _launch("drm_mx4_linear", device, x.data_ptr(), _row_stride(x), xid, codes.data_ptr(), scales.data_ptr(), ptr(bias), bid, y.data_ptr(), N,
-                M, N, K)
+                M, N, K, ptr(ws), need)
     return y
 
 
@@ -959,7 +963,9 @@ def mx4_linear_dgrad(dy, codes, scales, K: int) -> torch.Tensor:
         raise NativeError(f"mx4_linear_dgrad: gradient has {N} columns, the weight {codes.shape[0]} rows")
     dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
     if M and N:
-        _launch("drm_mx4_linear_dgrad", device, dy.data_ptr(), _row_stride(dy), yid, codes.data_ptr(), scales.data_ptr(), dx.data_ptr(), K, M, N, K)
+        ws, need = _workspace(dy.device, "drm_mx4_linear_dgrad_workspace_bytes", yid, M, N, K)
+        _launch("drm_mx4_linear_dgrad", device, dy.data_ptr(), _row_stride(dy), yid, codes.data_ptr(), scales.data_ptr(), dx.data_ptr(), K, M, N, K,
+                ptr(ws), need)
     return dx if N else dx.zero_()
 
 
@@ -988,6 +994,7 @@ def mx4_product(x_codes, x_scales, w_codes, w_scales, K: int, bias, dtype) -> to
     bid = _mx4_bias(bias, N, device, "mx4_product")
     y = torch.empty((M, N), dtype=dtype, device=x_codes.device)
     if M and N:
+        ws, need = _workspace(x_codes.device, "drm_mx4_product_workspace_bytes", M, N, K)
         _launch("drm_mx4_product", device, x_codes.data_ptr(), x_scales.data_ptr(), w_codes.data_ptr(), w_scales.data_ptr(), ptr(bias), bid,
-                y.data_ptr(), N, did, M, N, K)
+                y.data_ptr(), N, did, M, N, K, ptr(ws), need)
     return y

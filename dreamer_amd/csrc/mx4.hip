@@ -3,6 +3,7 @@
 
 #include <type_traits>
 
+#include <algorithm>
 #include <climits>
 
 namespace drm {
@@ -350,8 +351,10 @@ __device__ __forceinline__ u32x4 quad_transpose(u32x4 d, int q) {
 
 template <typename T, int BK, bool DIRECT, bool GRAD, bool RING>
 __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__ x, int64_t ldx, Mx4 W, const void* bias, int btype,
-                                                  T* __restrict__ y, int64_t ldy, int M, int N, int K, int tiles_m, int tiles_n) {
+                                                  T* __restrict__ y, int64_t ldy, int M, int N, int K, int tiles_m, int tiles_n,
+                                                  float* __restrict__ part, int span) {
     // y: reduction over W's columns (K of them), N = W's rows; dx: reduction over W's rows (K of them), N = W's columns
+    // With `part` the workgroups of blockIdx.y take `span` of the reduction each and leave (gridDim.y, M, N) fp32 sums there.
     static_assert(!DIRECT || Parts<T>::N == 1, "direct loads bring bf16");
     static_assert(!RING || (DIRECT && !GRAD), "a ring of stages has no loads through registers");
     using Stage = TileStage<T, BK, GRAD>;
@@ -364,6 +367,8 @@ __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__
     int tm, tn;
     mx4_tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
     const int m0 = tm * 128, n0 = tn * 128, wm = (wave & 1) * 64, wn = (wave >> 1) * WN;
+    const int begin = blockIdx.y * span;                          // a multiple of BK
+    K = min(K, begin + span);
     f32x16 acc[1][2];
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -519,14 +524,14 @@ __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__
     Held h;
     if constexpr (!GRAD && !RING) {
         if (W.nb >= NB) {
-            load_scales(0, h);
+            load_scales(begin, h);
         } else {                          // a row shorter than a step (then there is no second one)
             h.sw[0] = 0u;
             for (int i = 0; i < W.nb; ++i)
                 h.sw[0] |= (uint32_t)W.scales[(int64_t)min(n0 + (int)(threadIdx.x & 127), N - 1) * W.nb + i] << (8 * i);
         }
     }
-    const int steps = (whole + BK - 1) / BK;
+    const int steps = (max(whole - begin, 0) + BK - 1) / BK;
     if constexpr (RING) {
         // Three stages, filled by direct loads only (rows of whole steps of blocks: every row's four scale bytes of a step are an
         // aligned dword).  Stage i's loads are issued two steps ahead.  Before it is used, every wave waits until no more than the next
@@ -550,9 +555,9 @@ __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__
             issue(after, k0 + 2 * BK);
             compute(st);
         };
-        issue(s0, 0);
-        issue(s1, BK);
-        int k0 = 0;
+        issue(s0, begin);
+        issue(s1, begin + BK);
+        int k0 = begin;
         for (int p = 0; p < steps / 3; ++p, k0 += 3 * BK) {
             turn(s0, k0, s2);
             turn(s1, k0 + BK, s0);
@@ -561,11 +566,11 @@ __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__
         if (steps % 3 > 0) turn(s0, k0, s2);
         if (steps % 3 > 1) turn(s1, k0 + BK, s0);
     } else if (steps > 0) {
-        load(s0, 0, h, false);
-        put(s0, 0, h, false);
+        load(s0, begin, h, false);
+        put(s0, begin, h, false);
         __syncthreads();
         for (int p = 0; p < steps / 2; ++p) {
-            const int k1 = (2 * p + 1) * BK, k2 = k1 + BK;
+            const int k1 = begin + (2 * p + 1) * BK, k2 = k1 + BK;
             if constexpr (!GRAD) load_scales(k1, h);      // first: nothing behind it has to wait for the rest
             load(s1, k1, h, false);
             compute(s0);
@@ -580,15 +585,17 @@ __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__
         if (steps & 1) compute(s0);
     }
     if (!DIRECT && whole < K) {
-        const int k0 = whole / BK * BK;
-        if constexpr (!GRAD) { if (k0 > 0) load_scales(k0, h); }
+        const int k0 = max(whole / BK * BK, begin);
+        if constexpr (!GRAD) { if (k0 > begin) load_scales(k0, h); }
         load(s1, k0, h, true);
         put(s1, k0, h, true);
         __syncthreads();
         compute(s1);
     }
     __syncthreads();
-    mx4_store_tile<T, 64, WN>(reinterpret_cast<float*>(&s0) + wave * 32 * OUT_LD, acc, y, ldy, m0 + wm, n0 + wn, M, N, bias, btype);
+    float* strip = reinterpret_cast<float*>(&s0) + wave * 32 * OUT_LD;
+    if (part != nullptr) mx4_store_tile<float, 64, WN>(strip, acc, part + (int64_t)blockIdx.y * M * N, N, m0 + wm, n0 + wn, M, N, nullptr, 0);
+    else mx4_store_tile<T, 64, WN>(strip, acc, y, ldy, m0 + wm, n0 + wn, M, N, bias, btype);
 }
 
 // ---- both operands in 4 bits ----------------------------------------------------------------------------------------------
@@ -664,7 +671,8 @@ __device__ __forceinline__ void mx4_turn(const u32x4 (&b)[TM], const u32x4 (&a)[
 
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(256) void k_mx4_product(Mx4 X, Mx4 W, const void* bias, int btype, T* __restrict__ y, int64_t ldy, int tiles_m,
-                                                     int tiles_n) {
+                                                     int tiles_n, float* __restrict__ part, int span) {
+    // with `part` the workgroups of blockIdx.y take `span` steps of the reduction each and leave (gridDim.y, M, N) fp32 sums there
     static_assert((BM / WM) * (BN / WN) == 4, "four waves");
     constexpr int TM = WM / 32, TN = WN / 32;
     using Stage = ProductStage<BM, BN>;
@@ -719,31 +727,56 @@ __global__ __launch_bounds__(256) void k_mx4_product(Mx4 X, Mx4 W, const void* b
         __builtin_amdgcn_sched_barrier(0);
     };
     Bytes8 vx{0u, 0u}, vw{0u, 0u};
-    codes(s0, 0);
+    const int first = blockIdx.y * span, steps = min((W.nb + 7) / 8 - first, span);
+    codes(s0, first * 8);
     if (W.nb >= 8) {
-        scales(0, vx, vw);
-        put_scales(s0, 0, vx, vw);
+        scales(first * 8, vx, vw);
+        put_scales(s0, first * 8, vx, vw);
     } else {
         put(s0, mx4_short_row_scales(X, m0 + (threadIdx.x & (BM - 1))), mx4_short_row_scales(W, n0 + (threadIdx.x & (BN - 1))));
     }
     __syncthreads();
-    const int steps = (W.nb + 7) / 8;
     for (int p = 0; p < steps / 2; ++p) {
-        const int kb1 = p * 16 + 8, kb2 = kb1 + 8;
+        const int kb1 = (first + 2 * p + 1) * 8, kb2 = kb1 + 8;
         scales(kb1, vx, vw);
         codes(s1, kb1);
         compute(s0);
         put_scales(s1, kb1, vx, vw);
         __syncthreads();
         scales(kb2, vx, vw);
-        codes(s0, kb2);                     // behind the last step: zero blocks, not used
+        codes(s0, kb2);                     // behind the last step: not used
         compute(s1);
         put_scales(s0, kb2, vx, vw);
         __syncthreads();
     }
     if (steps & 1) compute(s0);
     __syncthreads();
-    mx4_store_tile<T, WM, WN>(reinterpret_cast<float*>(&s0) + wave * 32 * OUT_LD, acc, y, ldy, m0 + wm, n0 + wn, X.rows, W.rows, bias, btype);
+    float* strip = reinterpret_cast<float*>(&s0) + wave * 32 * OUT_LD;
+    if (part != nullptr) {
+        mx4_store_tile<float, WM, WN>(strip, acc, part + (int64_t)blockIdx.y * X.rows * W.rows, W.rows, m0 + wm, n0 + wn, X.rows, W.rows, nullptr, 0);
+        return;
+    }
+    mx4_store_tile<T, WM, WN>(strip, acc, y, ldy, m0 + wm, n0 + wn, X.rows, W.rows, bias, btype);
+}
+
+// sums of the slices of a split reduction, in order, + bias
+template <typename T>
+__global__ __launch_bounds__(256) void k_mx4_join(const float* __restrict__ part, int slices, int M, int N, const void* bias, int btype,
+                                                  T* __restrict__ y, int64_t ldy) {
+    const int64_t slots = ((int64_t)N + 3) / 4, total = (int64_t)M * slots, size = (int64_t)M * N;
+    for (int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x; o < total; o += (int64_t)gridDim.x * 256) {
+        const int64_t m = o / slots, n = (o - m * slots) * 4;
+        float v[4], u[4];
+        load_slot(part + m * N, n, N, 0.f, v);
+        for (int k = 1; k < slices; ++k) {
+            load_slot(part + k * size + m * N, n, N, 0.f, u);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += u[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < N) y[m * ldy + n + i] = (T)(v[i] + (bias != nullptr ? load_elem(bias, btype, n + i) : 0.f));
+    }
 }
 
 // ---- bias gradient: column sums of dy ----------------------------------------------------------------------------------
@@ -784,6 +817,7 @@ __global__ __launch_bounds__(256) void k_mx4_colsum_join(const float* __restrict
 }
 static inline int mx4_colsum_slices(int M) { return M <= 128 ? 1 : M <= 2048 ? (M + 127) / 128 : 16; }
 
+static inline int mx4_stream_grid(int64_t quads) { return (int)(quads < 256 * 16384ll ? (quads + 255) / 256 : 16384); }
 static inline int mx4_blocks(int K) { return K / 32 + (K % 32 != 0); }
 
 static int mx4_check(const char* what, const void* codes, const void* scales, int64_t rows, int32_t K) {
@@ -799,24 +833,44 @@ static int mx4_check_product(const char* what, const void* x, int64_t ldx, int d
                 "%s: M=%d N=%d, row strides %lld and %lld", what, M, out, (long long)ldx, (long long)ldy);
     return DRM_OK;
 }
+// A reduction is split over workgroups where the tiles alone leave CUs idle: into about one workgroup a CU, of four steps at
+// least.  Returns the number of slices and the steps of each.
+static inline int mx4_split(int64_t tiles, int steps, int& span) {
+    const int64_t want = tiles < 192 ? 256 / (tiles > 0 ? tiles : 1) : 1;
+    const int slices = (int)std::max<int64_t>(1, std::min<int64_t>(want, steps / 4));
+    span = (steps + slices - 1) / slices;
+    return (steps + span - 1) / span;
+}
+static inline int64_t mx4_tiles(int M, int N, int b) { return (int64_t)((M + b - 1) / b) * ((N + b - 1) / b); }
+static inline size_t mx4_part_bytes(int slices, int M, int N) { return slices > 1 ? (size_t)slices * M * N * sizeof(float) : 0; }
+static inline int mx4_step_of(int dtype) { return dtype == DRM_BF16 ? 128 : 64; }
+
 // Large products: bf16 rows whose 16-byte chunks are aligned and whole go to LDS by direct loads with 128 of the reduction per step
 // (three stages where a row's scales are whole dwords); through registers the parts of wider types leave room for 64.
 template <bool GRAD, typename T>
-static void mx4_launch_tile(const T* x, int64_t ldx, const Mx4& W, const void* bias, int btype, T* y, int64_t ldy, int M, int N, int K, hipStream_t s) {
+static void mx4_launch_tile(const T* x, int64_t ldx, const Mx4& W, const void* bias, int btype, T* y, int64_t ldy, int M, int N, int K,
+                            float* part, hipStream_t s) {
     const int tm = (M + 127) / 128, tn = (N + 127) / 128;
+    constexpr int BK = Parts<T>::N == 1 ? 128 : 64;
+    int span = 0;
+    const int slices = mx4_split((int64_t)tm * tn, (K + BK - 1) / BK, span);
+    if (slices == 1) part = nullptr;
+    const dim3 grid(tm * tn, slices);
+    auto go = [&](auto direct, auto ring) {
+        constexpr bool DIRECT = decltype(direct)::value, RING = decltype(ring)::value;
+        k_mx4_tile<T, BK, DIRECT, GRAD, RING><<<grid, TILE_THREADS, 0, s>>>(x, ldx, W, bias, btype, y, ldy, M, N, K, tm, tn, part, span * BK);
+    };
+    bool done = false;
     if constexpr (Parts<T>::N == 1) {
         if (aligned16(x) && ldx % 8 == 0 && K % 8 == 0 && ldx <= (1 << 22)) {
             if constexpr (!GRAD) {
-                if (W.nb % 4 == 0 && ((uintptr_t)W.scales & 3) == 0) {
-                    k_mx4_tile<T, 128, true, false, true><<<tm * tn, TILE_THREADS, 0, s>>>(x, ldx, W, bias, btype, y, ldy, M, N, K, tm, tn);
-                    return;
-                }
+                if (W.nb % 4 == 0 && ((uintptr_t)W.scales & 3) == 0) { go(std::true_type{}, std::true_type{}); done = true; }
             }
-            k_mx4_tile<T, 128, true, GRAD, false><<<tm * tn, TILE_THREADS, 0, s>>>(x, ldx, W, bias, btype, y, ldy, M, N, K, tm, tn);
-            return;
+            if (!done) { go(std::true_type{}, std::false_type{}); done = true; }
         }
     }
-    k_mx4_tile<T, Parts<T>::N == 1 ? 128 : 64, false, GRAD, false><<<tm * tn, TILE_THREADS, 0, s>>>(x, ldx, W, bias, btype, y, ldy, M, N, K, tm, tn);
+    if (!done) go(std::false_type{}, std::false_type{});
+    if (part != nullptr) k_mx4_join<T><<<mx4_stream_grid((int64_t)M * ((N + 3) / 4)), 256, 0, s>>>(part, slices, M, N, bias, btype, y, ldy);
 }
 // Few rows: as many weight tiles per wave as leave about one workgroup a CU (x is read once per workgroup); eight waves where two
 // stages of their passes fit the LDS, else four.
@@ -850,7 +904,6 @@ static int mx4_check_tiles(const char* what, int M, int N, int K) {
     DRM_REQUIRE(((int64_t)M + 127) / 128 * (((int64_t)N + 127) / 128) <= INT_MAX / 4, DRM_ENOTSUP, "%s: M=%d N=%d: too many tiles", what, M, N);
     return DRM_OK;
 }
-static inline int mx4_stream_grid(int64_t quads) { return (int)(quads < 256 * 16384ll ? (quads + 255) / 256 : 16384); }
 
 }  // namespace drm
 
@@ -890,37 +943,68 @@ extern "C" int drm_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, i
     });
 }
 
+// the largest tile (fewest bytes through LDS per product) whose tiles still give most CUs one
+static int mx4_product_tile(int M, int N) { return mx4_tiles(M, N, 256) >= 192 ? 256 : mx4_tiles(M, N, 128) >= 192 ? 128 : 64; }
+
+static int mx4_check_workspace(const char* what, const void* ws, size_t have, size_t need) {
+    DRM_REQUIRE(need == 0 || (ws && have >= need && aligned16(ws)), DRM_EINVAL, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", what,
+                ws ? have : (size_t)0, need);
+    return DRM_OK;
+}
+
+extern "C" size_t drm_mx4_linear_workspace_bytes(int32_t dtype, int32_t M, int32_t N, int32_t K) {
+    if (!elem_ok(dtype) || M <= MX4_FEW_ROWS || N < 1 || K < 1) return 0;
+    int span = 0;
+    const int bk = mx4_step_of(dtype);
+    return mx4_part_bytes(mx4_split(mx4_tiles(M, N, 128), (K - 1) / bk + 1, span), M, N);
+}
+extern "C" size_t drm_mx4_linear_dgrad_workspace_bytes(int32_t dtype, int32_t M, int32_t N, int32_t K) {
+    if (!elem_ok(dtype) || M < 1 || N < 1 || K < 1) return 0;
+    int span = 0;
+    const int bk = mx4_step_of(dtype);
+    return mx4_part_bytes(mx4_split(mx4_tiles(M, K, 128), (N - 1) / bk + 1, span), M, K);
+}
+extern "C" size_t drm_mx4_product_workspace_bytes(int32_t M, int32_t N, int32_t K) {
+    if (M < 1 || N < 1 || K < 1) return 0;
+    int span = 0;
+    return mx4_part_bytes(mx4_split(mx4_tiles(M, N, mx4_product_tile(M, N)), (mx4_blocks(K) + 7) / 8, span), M, N);
+}
+
 extern "C" int drm_mx4_linear(const void* x, int64_t ldx, int32_t dtype, const uint8_t* codes, const uint8_t* scales, const void* bias,
-                              int32_t bias_dtype, void* y, int64_t ldy, int32_t M, int32_t N, int32_t K, drm_stream_t stream) {
+                              int32_t bias_dtype, void* y, int64_t ldy, int32_t M, int32_t N, int32_t K, void* workspace,
+                              size_t workspace_bytes, drm_stream_t stream) {
     if (M == 0 && N >= 1 && K >= 1) return DRM_OK;
     if (int rc = mx4_check(__func__, codes, scales, N, K)) return rc;
     if (int rc = mx4_check_product(__func__, x, ldx, dtype, K, bias, bias_dtype, y, ldy, N, M)) return rc;
     if (int rc = mx4_check_tiles(__func__, M, N, K)) return rc;
+    if (int rc = mx4_check_workspace(__func__, workspace, workspace_bytes, drm_mx4_linear_workspace_bytes(dtype, M, N, K))) return rc;
     hipStream_t s = (hipStream_t)stream;
     const Mx4 W{codes, scales, N, mx4_blocks(K)};
     ProfScope ps(M <= MX4_FEW_ROWS ? PC_LINEAR : PC_LINEAR_BIG, s, 2.0 * M * N * K, ((double)M * K + (double)M * N) * elem_bytes(dtype) + (double)N * W.nb * 17);
     return with_elem(dtype, [&](auto tag) -> int {
         using T = decltype(tag);
         if (M <= MX4_FEW_ROWS) mx4_launch_rows<T>((const T*)x, ldx, W, bias, bias_dtype, (T*)y, ldy, M, N, K, s);
-        else mx4_launch_tile<false, T>((const T*)x, ldx, W, bias, bias_dtype, (T*)y, ldy, M, N, K, s);
+        else mx4_launch_tile<false, T>((const T*)x, ldx, W, bias, bias_dtype, (T*)y, ldy, M, N, K, (float*)workspace, s);
         DRM_LAUNCH_CHECK();
         return DRM_OK;
     });
 }
 
 extern "C" int drm_mx4_linear_dgrad(const void* dy, int64_t lddy, int32_t dtype, const uint8_t* codes, const uint8_t* scales, void* dx,
-                                    int64_t lddx, int32_t M, int32_t N, int32_t K, drm_stream_t stream) {
+                                    int64_t lddx, int32_t M, int32_t N, int32_t K, void* workspace, size_t workspace_bytes,
+                                    drm_stream_t stream) {
     if (M == 0 && N >= 1 && K >= 1) return DRM_OK;
     if (int rc = mx4_check(__func__, codes, scales, N, K)) return rc;
     if (int rc = mx4_check_product(__func__, dy, lddy, dtype, N, nullptr, 0, dx, lddx, K, M)) return rc;
     if (int rc = mx4_check_tiles(__func__, M, K, K)) return rc;
     DRM_REQUIRE(N >= 1, DRM_EINVAL, "N=%d", N);
+    if (int rc = mx4_check_workspace(__func__, workspace, workspace_bytes, drm_mx4_linear_dgrad_workspace_bytes(dtype, M, N, K))) return rc;
     hipStream_t s = (hipStream_t)stream;
     const Mx4 W{codes, scales, N, mx4_blocks(K)};
     ProfScope ps(PC_LINEAR_BIG, s, 2.0 * M * N * K, ((double)M * K + (double)M * N) * elem_bytes(dtype) + (double)N * W.nb * 17);
     return with_elem(dtype, [&](auto tag) -> int {
         using T = decltype(tag);
-        mx4_launch_tile<true, T>((const T*)dy, lddy, W, nullptr, 0, (T*)dx, lddx, M, K, N, s);
+        mx4_launch_tile<true, T>((const T*)dy, lddy, W, nullptr, 0, (T*)dx, lddx, M, K, N, (float*)workspace, s);
         DRM_LAUNCH_CHECK();
         return DRM_OK;
     });
@@ -928,29 +1012,27 @@ extern "C" int drm_mx4_linear_dgrad(const void* dy, int64_t lddy, int32_t dtype,
 
 extern "C" int drm_mx4_product(const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales,
                                const void* bias, int32_t bias_dtype, void* y, int64_t ldy, int32_t y_dtype, int32_t M, int32_t N,
-                               int32_t K, drm_stream_t stream) {
+                               int32_t K, void* workspace, size_t workspace_bytes, drm_stream_t stream) {
     if (M == 0 && N >= 1 && K >= 1) return DRM_OK;
     if (int rc = mx4_check(__func__, x_codes, x_scales, M, K)) return rc;
     if (int rc = mx4_check(__func__, w_codes, w_scales, N, K)) return rc;
     if (int rc = mx4_check_product(__func__, x_codes, K, y_dtype, K, bias, bias_dtype, y, ldy, N, M)) return rc;
     if (int rc = mx4_check_tiles(__func__, M, N, K)) return rc;
+    if (int rc = mx4_check_workspace(__func__, workspace, workspace_bytes, drm_mx4_product_workspace_bytes(M, N, K))) return rc;
     hipStream_t s = (hipStream_t)stream;
     const Mx4 X{x_codes, x_scales, M, mx4_blocks(K)}, W{w_codes, w_scales, N, mx4_blocks(K)};
     ProfScope ps(PC_LINEAR_BIG, s, 2.0 * M * N * K, (double)M * N * elem_bytes(y_dtype) + ((double)M + N) * W.nb * 17);
     return with_elem(y_dtype, [&](auto tag) -> int {
         using T = decltype(tag);
-        // the largest tile (fewest bytes through LDS per product) whose tiles still give every CU one
-        auto tiles = [&](int b) { return (int64_t)((M + b - 1) / b) * ((N + b - 1) / b); };
-        if (tiles(256) >= 192) {
-            const int tm = (M + 255) / 256, tn = (N + 255) / 256;
-            k_mx4_product<T, 256, 256, 128, 128><<<tm * tn, 256, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy, tm, tn);
-        } else if (tiles(128) >= 192) {
-            const int tm = (M + 127) / 128, tn = (N + 127) / 128;
-            k_mx4_product<T, 128, 128, 64, 64><<<tm * tn, 256, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy, tm, tn);
-        } else {
-            const int tm = (M + 63) / 64, tn = (N + 63) / 64;
-            k_mx4_product<T, 64, 64, 32, 32><<<tm * tn, 256, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy, tm, tn);
-        }
+        const int b = mx4_product_tile(M, N), tm = (M + b - 1) / b, tn = (N + b - 1) / b;
+        int span = 0;
+        const int slices = mx4_split((int64_t)tm * tn, (W.nb + 7) / 8, span);
+        float* part = slices > 1 ? (float*)workspace : nullptr;
+        const dim3 grid(tm * tn, slices);
+        if (b == 256) k_mx4_product<T, 256, 256, 128, 128><<<grid, 256, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy, tm, tn, part, span);
+        else if (b == 128) k_mx4_product<T, 128, 128, 64, 64><<<grid, 256, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy, tm, tn, part, span);
+        else k_mx4_product<T, 64, 64, 32, 32><<<grid, 256, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy, tm, tn, part, span);
+        if (part != nullptr) k_mx4_join<T><<<mx4_stream_grid((int64_t)M * ((N + 3) / 4)), 256, 0, s>>>(part, slices, M, N, bias, bias_dtype, (T*)y, ldy);
         DRM_LAUNCH_CHECK();
         return DRM_OK;
     });

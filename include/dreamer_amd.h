@@ -575,16 +575,23 @@ int drm_mx4_quantize(const void* x, int64_t ldx, int32_t dtype, int64_t rows, in
                      drm_stream_t stream);
 int drm_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int32_t K, void* y, int64_t ldy, int32_t dtype,
                        drm_stream_t stream);
+/* the products split the reduction over workgroups where the outputs are few: `workspace` of *_workspace_bytes (may be 0), 16-byte
+ * aligned; the slices are added in a fixed order */
+size_t drm_mx4_linear_workspace_bytes(int32_t dtype, int32_t M, int32_t N, int32_t K);
 int drm_mx4_linear(const void* x, int64_t ldx, int32_t dtype, const uint8_t* codes, const uint8_t* scales, const void* bias,
-                   int32_t bias_dtype, void* y, int64_t ldy, int32_t M, int32_t N, int32_t K, drm_stream_t stream);
+                   int32_t bias_dtype, void* y, int64_t ldy, int32_t M, int32_t N, int32_t K, void* workspace, size_t workspace_bytes,
+                   drm_stream_t stream);
+size_t drm_mx4_linear_dgrad_workspace_bytes(int32_t dtype, int32_t M, int32_t N, int32_t K);
 int drm_mx4_linear_dgrad(const void* dy, int64_t lddy, int32_t dtype, const uint8_t* codes, const uint8_t* scales, void* dx,
-                         int64_t lddx, int32_t M, int32_t N, int32_t K, drm_stream_t stream);
+                         int64_t lddx, int32_t M, int32_t N, int32_t K, void* workspace, size_t workspace_bytes, drm_stream_t stream);
 /* bias gradient of `linear`: column sums of dy (M, N) in db_dtype, added in fp32 in an order that depends on M and N only */
 size_t drm_mx4_bias_grad_workspace_bytes(int32_t M, int32_t N);
 int drm_mx4_bias_grad(const void* dy, int64_t lddy, int32_t dtype, void* db, int32_t db_dtype, int32_t M, int32_t N, void* workspace,
                       size_t workspace_bytes, drm_stream_t stream);
+size_t drm_mx4_product_workspace_bytes(int32_t M, int32_t N, int32_t K);
 int drm_mx4_product(const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales, const void* bias,
-                    int32_t bias_dtype, void* y, int64_t ldy, int32_t y_dtype, int32_t M, int32_t N, int32_t K, drm_stream_t stream);
+                    int32_t bias_dtype, void* y, int64_t ldy, int32_t y_dtype, int32_t M, int32_t N, int32_t K, void* workspace,
+                    size_t workspace_bytes, drm_stream_t stream);
 
 #ifdef __cplusplus
 }

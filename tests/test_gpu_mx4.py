@@ -124,7 +124,7 @@ def _bound(x, w, b, y, K, parts, dtype):
 
 PARTS = {F32: 3, BF16: 1, F16: 2}
 SHAPES = [(1, 1, 1), (1, 16, 32), (2, 17, 33), (15, 40, 100), (16, 1000, 512), (17, 31, 96), (33, 130, 257), (64, 128, 128), (65, 129, 65),
-          (128, 64, 31), (129, 200, 1000), (300, 257, 130), (257, 384, 4080)]
+          (128, 64, 31), (129, 200, 1000), (300, 257, 130), (257, 384, 4080), (40, 100, 2053), (100, 64, 8200), (130, 2051, 72)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])

@@ -88,7 +88,7 @@ def test_mx4_entry_points_refuse():
     assert L.drm_mx4_quantize(None, 32, 0, 0, 32, None, None, None) == 0
     _err(L.drm_mx4_dequantize(P, P, 4, 32, None, 32, 0, None), EINVAL, "null")
     _err(L.drm_mx4_dequantize(P, P, 4, 32, P, 31, 0, None), EINVAL, "stride")
-    lin = lambda x=P, ldx=32, dt=0, c=P, s=P, b=None, bt=0, y=P, ldy=8, M=4, n=8, K=32: L.drm_mx4_linear(x, ldx, dt, c, s, b, bt, y, ldy, M, n, K, None)
+    lin = lambda x=P, ldx=32, dt=0, c=P, s=P, b=None, bt=0, y=P, ldy=8, M=4, n=8, K=32, ws=P, nb=1 << 40: L.drm_mx4_linear(x, ldx, dt, c, s, b, bt, y, ldy, M, n, K, ws, nb, None)
     for kw in (dict(x=None), dict(c=None), dict(s=None), dict(y=None)):
         _err(lin(**kw), EINVAL, "null")
     _err(lin(ldx=31), EINVAL, "stride")
@@ -99,14 +99,18 @@ def test_mx4_entry_points_refuse():
     _err(lin(n=0, ldy=0), EINVAL, "N=0")
     _err(lin(M=2 ** 31 - 300), ENOTSUP, "at most")
     assert lin(M=0) == 0
+    need = L.drm_mx4_linear_workspace_bytes(0, 100, 128, 4096)
+    assert need > 0 and L.drm_mx4_linear_workspace_bytes(0, 4, 128, 4096) == 0 and L.drm_mx4_linear_workspace_bytes(9, 100, 128, 4096) == 0
+    for ws, nb in ((None, 0), (P, need - 1), (P + 8, need)):
+        _err(lin(M=100, n=128, K=4096, ldx=4096, ldy=128, ws=ws, nb=nb), EINVAL, "workspace")
     grad = lambda **kw: L.drm_mx4_linear_dgrad(*[dict(dict(dy=P, ld=8, dt=0, c=P, s=P, dx=P, ldx=32, M=4, N=8, K=32), **kw)[k] for k in
-                                                 ("dy", "ld", "dt", "c", "s", "dx", "ldx", "M", "N", "K")], None)
+                                                 ("dy", "ld", "dt", "c", "s", "dx", "ldx", "M", "N", "K")], P, 1 << 40, None)
     for kw in (dict(dy=None), dict(dx=None), dict(c=None)):
         _err(grad(**kw), EINVAL, "null")
     _err(grad(ld=7), EINVAL, "stride")
     _err(grad(ldx=31), EINVAL, "stride")
     prod = lambda **kw: L.drm_mx4_product(*[dict(dict(a=P, sa=P, w=P, sw=P, b=None, bt=0, y=P, ldy=8, yt=0, M=4, N=8, K=32), **kw)[k] for k in
-                                            ("a", "sa", "w", "sw", "b", "bt", "y", "ldy", "yt", "M", "N", "K")], None)
+                                            ("a", "sa", "w", "sw", "b", "bt", "y", "ldy", "yt", "M", "N", "K")], P, 1 << 40, None)
     for kw in (dict(a=None), dict(sa=None), dict(w=None), dict(sw=None), dict(y=None)):
         _err(prod(**kw), EINVAL, "null")
     _err(prod(ldy=7), EINVAL, "stride")
