@@ -599,7 +599,7 @@ __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__
 }
 
 // ---- both operands in 4 bits ----------------------------------------------------------------------------------------------
-// Tiles of BM x BN outputs, 256 deep per step (eight blocks, 128 bytes a row), four waves, each owning WM x WN of 32x32x64 scaled
+// Tiles of BM x BN outputs, 256 deep per step (eight blocks, 128 bytes a row), waves of WM x WN in 32x32x64 scaled
 // matrix instructions.  The codes go from memory to LDS as they are (16-byte direct loads, no registers in between), two buffers:
 // the loads of the next step run under the matrix instructions of this one.  A direct load fills LDS in lane order, so the lanes
 // choose their source instead: slot p of row r holds block p ^ (r / 2 & 7): a fragment read takes 16 rows a clock, which then fall on all 64 banks.
@@ -613,10 +613,10 @@ struct ProductStage {
     __attribute__((aligned(16))) uint8_t x[BM * 128];
     __attribute__((aligned(16))) uint8_t w[BN * 128];
     uint32_t sx[BM * 2], sw[BN * 2];
-    uint32_t room[256];                  // (the 64 x 64 tile's output strips are a little longer than its codes)
+    uint32_t room[512];                  // (the output strips of the smaller tiles are a little longer than their codes)
 };
 
-template <int ROWS>
+template <int ROWS, int WAVES>
 __device__ __forceinline__ void mx4_stage_codes(const Mx4& A, int r0, int kb0, uint8_t* lds) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int lr = wave * 8 + (lane >> 3);
@@ -624,11 +624,11 @@ __device__ __forceinline__ void mx4_stage_codes(const Mx4& A, int r0, int kb0, u
     const int c = (lane & 7) ^ (((wave * 8 + (lane >> 3)) >> 1) & 7), last = A.rows - 1 - r0;
     const uint8_t* base = A.codes + ((int64_t)r0 * A.nb + kb0) * 16;      // offsets inside a tile stay below 2^31 (checked at the call)
 #pragma unroll
-    for (int j = 0; j < ROWS / 32; ++j) {
-        const uint8_t* src = base + (uint32_t)((min(lr + j * 32, last) * A.nb + c) * 16);
+    for (int j = 0; j < ROWS / (8 * WAVES); ++j) {
+        const uint8_t* src = base + (uint32_t)((min(lr + j * 8 * WAVES, last) * A.nb + c) * 16);
         src = kb0 + c < A.nb ? src : reinterpret_cast<const uint8_t*>(&mx4_zero_block);
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src,
-                                         (__attribute__((address_space(3))) uint32_t*)(lds + (j * 4 + wave) * 1024), 16, 0, 0);
+                                         (__attribute__((address_space(3))) uint32_t*)(lds + (j * WAVES + wave) * 1024), 16, 0, 0);
     }
 }
 // the scale bytes of a row's blocks [kb0, kb0 + 8), 0 behind the last one; nb >= 8 (no branch: the row's last eight, shifted when
@@ -670,14 +670,14 @@ __device__ __forceinline__ void mx4_turn(const u32x4 (&b)[TM], const u32x4 (&a)[
 }
 
 template <typename T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(256) void k_mx4_product(Mx4 X, Mx4 W, const void* bias, int btype, T* __restrict__ y, int64_t ldy, int tiles_m,
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void k_mx4_product(Mx4 X, Mx4 W, const void* bias, int btype, T* __restrict__ y, int64_t ldy, int tiles_m,
                                                      int tiles_n, float* __restrict__ part, int span) {
     // with `part` the workgroups of blockIdx.y take `span` steps of the reduction each and leave (gridDim.y, M, N) fp32 sums there
-    static_assert((BM / WM) * (BN / WN) == 4, "four waves");
+    constexpr int WAVES = (BM / WM) * (BN / WN), THREADS = WAVES * 64;
     constexpr int TM = WM / 32, TN = WN / 32;
     using Stage = ProductStage<BM, BN>;
     constexpr int OUT_LD = WN + 4;                                // floats per row of the output strip
-    static_assert(sizeof(Stage) >= 4 * 32 * OUT_LD * sizeof(float), "the output strips fit one stage");
+    static_assert(sizeof(Stage) >= WAVES * 32 * OUT_LD * sizeof(float), "the output strips fit one stage");
     __shared__ Stage s0, s1;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int tm, tn;
@@ -690,19 +690,30 @@ __global__ __launch_bounds__(256) void k_mx4_product(Mx4 X, Mx4 W, const void* b
         for (int j = 0; j < TM; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    // scales: thread t brings row t of the x tile and row t of the w tile
+    // scales: a thread brings those of one row of each tile, or of one of them where the threads suffice (smaller tiles: more than once)
+    constexpr bool HALVES = THREADS >= BM + BN;
+    const bool second = HALVES && threadIdx.x >= THREADS / 2;
+    const int rx = threadIdx.x & (BM - 1), rw = threadIdx.x & (BN - 1);
     auto scales = [&](int kb0, Bytes8& vx, Bytes8& vw) {
-        vx = mx4_row_scales(X, m0 + (threadIdx.x & (BM - 1)), kb0);
-        vw = mx4_row_scales(W, n0 + (threadIdx.x & (BN - 1)), kb0);
+        if constexpr (HALVES) {
+            vx = second ? mx4_row_scales(W, n0 + rw, kb0) : mx4_row_scales(X, m0 + rx, kb0);
+        } else {
+            vx = mx4_row_scales(X, m0 + rx, kb0);
+            vw = mx4_row_scales(W, n0 + rw, kb0);
+        }
     };
     auto put = [&](Stage& st, uint2 vx, uint2 vw) {
-        *reinterpret_cast<uint2*>(&st.sx[(threadIdx.x & (BM - 1)) * 2]) = vx;      // (smaller tiles: the same value more than once)
-        *reinterpret_cast<uint2*>(&st.sw[(threadIdx.x & (BN - 1)) * 2]) = vw;
+        if constexpr (HALVES) {
+            *reinterpret_cast<uint2*>(second ? &st.sw[rw * 2] : &st.sx[rx * 2]) = vx;
+        } else {
+            *reinterpret_cast<uint2*>(&st.sx[rx * 2]) = vx;
+            *reinterpret_cast<uint2*>(&st.sw[rw * 2]) = vw;
+        }
     };
     auto put_scales = [&](Stage& st, int kb0, Bytes8 vx, Bytes8 vw) { put(st, mx4_shift_scales(vx, W.nb, kb0), mx4_shift_scales(vw, W.nb, kb0)); };
     auto codes = [&](Stage& st, int kb0) {
-        mx4_stage_codes<BM>(X, m0, kb0, st.x);
-        mx4_stage_codes<BN>(W, n0, kb0, st.w);
+        mx4_stage_codes<BM, WAVES>(X, m0, kb0, st.x);
+        mx4_stage_codes<BN, WAVES>(W, n0, kb0, st.w);
     };
     auto compute = [&](const Stage& st) {
         int sx[TM], sw[TN];
@@ -733,7 +744,8 @@ __global__ __launch_bounds__(256) void k_mx4_product(Mx4 X, Mx4 W, const void* b
         scales(first * 8, vx, vw);
         put_scales(s0, first * 8, vx, vw);
     } else {
-        put(s0, mx4_short_row_scales(X, m0 + (threadIdx.x & (BM - 1))), mx4_short_row_scales(W, n0 + (threadIdx.x & (BN - 1))));
+        const uint2 sx = mx4_short_row_scales(X, m0 + rx), sw = mx4_short_row_scales(W, n0 + rw);
+        put(s0, second ? sw : sx, sw);
     }
     __syncthreads();
     for (int p = 0; p < steps / 2; ++p) {
@@ -1029,8 +1041,8 @@ extern "C" int drm_mx4_product(const uint8_t* x_codes, const uint8_t* x_scales, 
         const int slices = mx4_split((int64_t)tm * tn, (W.nb + 7) / 8, span);
         float* part = slices > 1 ? (float*)workspace : nullptr;
         const dim3 grid(tm * tn, slices);
-        if (b == 256) k_mx4_product<T, 256, 256, 128, 128><<<grid, 256, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy, tm, tn, part, span);
-        else if (b == 128) k_mx4_product<T, 128, 128, 64, 64><<<grid, 256, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy, tm, tn, part, span);
+        if (b == 256) k_mx4_product<T, 256, 256, 128, 64><<<grid, 512, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy, tm, tn, part, span);
+        else if (b == 128) k_mx4_product<T, 128, 128, 64, 32><<<grid, 512, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy, tm, tn, part, span);
         else k_mx4_product<T, 64, 64, 32, 32><<<grid, 256, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy, tm, tn, part, span);
         if (part != nullptr) k_mx4_join<T><<<mx4_stream_grid((int64_t)M * ((N + 3) / 4)), 256, 0, s>>>(part, slices, M, N, bias, bias_dtype, (T*)y, ldy);
         DRM_LAUNCH_CHECK();
