@@ -53,32 +53,21 @@ __global__ __launch_bounds__(256) void k_mx4_quantize(const T* __restrict__ x, i
     }
 }
 
+// A lane writes one 16-byte slot of the row (VEC codes).
 template <typename T>
 __global__ __launch_bounds__(256) void k_mx4_dequantize(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows,
                                                         int K, int nb, T* __restrict__ y, int64_t ldy) {
-    const int64_t quads = rows * nb * 4, step = (int64_t)gridDim.x * 256;
-    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < quads; q += step) {
-        const int64_t blk = q >> 2, r = blk / nb;
-        const int64_t at = (blk - r * nb) * 32 + (q & 3) * 8;
-        const uint32_t c = reinterpret_cast<const uint32_t*>(codes)[q];
-        const uint32_t s = scales[blk];
-        float v[8];
+    constexpr int VEC = Elem<T>::VEC, PER = 32 / VEC;
+    using Codes = std::conditional_t<VEC == 8, uint32_t, uint16_t>;
+    const int64_t slots = rows * nb * PER, step = (int64_t)gridDim.x * 256;
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < slots; q += step) {
+        const int64_t blk = q / PER, r = blk / nb;
+        // bf16 holds every value; below 2^128 so do fp32 and, inside its range, fp16
+        const bf16x8 h = mx4_bf16x8((uint32_t)reinterpret_cast<const Codes*>(codes)[q], mx4_scale(scales[blk]));
+        float v[VEC];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            // e2m1 as an integer: magnitudes 0, 1, 2, 3, 4, 6, 8, 12 halves
-            const uint32_t m = (c >> (4 * i)) & 7u;
-            const float h = (float)(m < 2 ? m : (2u | (m & 1u)) << ((m >> 1) - 1));
-            const float a = s == 255u ? __builtin_bit_cast(float, 0x7fc00000u) : ldexpf(h, (int)s - 128);
-            v[i] = (c >> (4 * i)) & 8u ? -a : a;
-        }
-        T* row = y + r * ldy;
-        if constexpr (Elem<T>::VEC == 8) {
-            store_slot(row, at, K, v);
-        } else {
-            const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
-            store_slot(row, at, K, a);
-            store_slot(row, at + 4, K, b);
-        }
+        for (int i = 0; i < VEC; ++i) v[i] = (float)h[i];
+        store_slot(y + r * ldy, (blk - r * nb) * 32 + (q % PER) * VEC, K, v);
     }
 }
 
@@ -949,7 +938,7 @@ extern "C" int drm_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, i
     ProfScope ps(PC_ELEMENTWISE, s, 2.0 * rows * K, (double)rows * K * elem_bytes(dtype) + (double)rows * nb * 17);
     return with_elem(dtype, [&](auto tag) -> int {
         using T = decltype(tag);
-        k_mx4_dequantize<T><<<mx4_stream_grid(rows * nb * 4), 256, 0, s>>>(codes, scales, rows, K, nb, (T*)y, ldy);
+        k_mx4_dequantize<T><<<mx4_stream_grid(rows * nb * (32 / Elem<T>::VEC)), 256, 0, s>>>(codes, scales, rows, K, nb, (T*)y, ldy);
         DRM_LAUNCH_CHECK();
         return DRM_OK;
     });
