@@ -182,17 +182,40 @@ __global__ __launch_bounds__(TPB) void k_distill_fwd(DistillArgs A, float c) {
     float m = -INFINITY, z = 0.f;
     for (int at = threadIdx.x * VEC; at < n; at += TPB * VEC * GROUP) {
         float v[GROUP][VEC];
+        if (n >= VEC) {
+            // all loads first; what is not a slot's own (see raw_slot) and what is listed does not count
+            Slot<T> raw[GROUP];
+            uint32_t dead[GROUP];
 #pragma unroll
-        for (int u = 0; u < GROUP; ++u) load_slot(row, at + u * TPB * VEC, n, -INFINITY, v[u]);
-        if (mask) {
+            for (int u = 0; u < GROUP; ++u) raw[u] = raw_slot(row, at + u * TPB * VEC, n);
+            uint32_t any = 0;
 #pragma unroll
             for (int u = 0; u < GROUP; ++u) {
-                const int o = at + u * TPB * VEC;
-                const uint32_t b = o < n ? (s_bits[o >> 5] >> (o & 31)) & ((1u << VEC) - 1u) : 0u;
-                if (b != 0) {
+                const int o = at + u * TPB * VEC, foreign = min(o - (int)slot_at<T>(o, n), VEC);
+                dead[u] = (1u << foreign) - 1u;
+                if (mask && o < n) dead[u] |= (s_bits[o >> 5] >> (o & 31)) << foreign;
+                dead[u] &= (1u << VEC) - 1u;
+                any |= dead[u];
+            }
+#pragma unroll
+            for (int u = 0; u < GROUP; ++u)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) v[u][i] = (float)raw[u].v[i];
+            if (any != 0) {
+#pragma unroll
+                for (int u = 0; u < GROUP; ++u)
 #pragma unroll
                     for (int i = 0; i < VEC; ++i)
-                        if ((b >> i) & 1u) v[u][i] = -INFINITY;
+                        if ((dead[u] >> i) & 1u) v[u][i] = -INFINITY;
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < GROUP; ++u) {
+                load_slot(row, at + u * TPB * VEC, n, -INFINITY, v[u]);
+                if (mask && u == 0) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i)
+                        if ((s_bits[0] >> (at + i)) & 1u) v[u][i] = -INFINITY;
                 }
             }
         }
@@ -266,16 +289,27 @@ __global__ __launch_bounds__(TPB) void k_distill_bwd(DistillBwdArgs A, float c) 
     const float g = live ? A.g[r] * A.inv_t : 0.f;
     const float fo = g * R.outside, fi = g * R.inside;
     for (int at = threadIdx.x * VEC; at < n; at += TPB * VEC * GROUP) {
-        float v[GROUP][VEC];
-        if (live) {
+        if (n >= VEC) {
+            // (a slot that was moved back writes some of its neighbour's results once more)
+            Slot<T> raw[GROUP];
+            if (live) {
 #pragma unroll
-            for (int u = 0; u < GROUP; ++u) load_slot(row, at + u * TPB * VEC, n, -INFINITY, v[u]);
-        }
+                for (int u = 0; u < GROUP; ++u) raw[u] = raw_slot(row, at + u * TPB * VEC, n);
+            }
 #pragma unroll
-        for (int u = 0; u < GROUP; ++u) {
+            for (int u = 0; u < GROUP; ++u) {
+                const int o = at + u * TPB * VEC;
+                Slot<T> r;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) v[u][i] = live ? exp_scaled(v[u][i] - R.m_out, c) * fo : 0.f;
-            if (at + u * TPB * VEC < n) store_slot(out, at + u * TPB * VEC, n, v[u]);
+                for (int i = 0; i < VEC; ++i) r.v[i] = (T)(live ? exp_scaled((float)raw[u].v[i] - R.m_out, c) * fo : 0.f);
+                if (o < n) *reinterpret_cast<Slot<T>*>(out + slot_at<T>(o, n)) = r;
+            }
+        } else {
+            float v[VEC];
+            if (live) load_slot(row, at, n, -INFINITY, v);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = live ? exp_scaled(v[i] - R.m_out, c) * fo : 0.f;
+            store_slot(out, at, n, v);
         }
     }
     if (!live) return;
