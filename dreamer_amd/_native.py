@@ -774,6 +774,12 @@ def dtype_id(t: torch.Tensor, name: str) -> int:
     return i
 
 
+def _sizes32(*sizes: int) -> None:
+    """The entry points take row lengths and product extents as 32-bit integers."""
+    if max(sizes) >= 1 << 31:
+        raise NativeError(f"an extent of {max(sizes)} elements: this operation takes rows and products of less than 2**31")
+
+
 def as_rows(x: torch.Tensor) -> torch.Tensor:
     """x as a matrix over its last dimension whose columns are contiguous and whose rows do not overlap (a view where it can be)."""
     if x.dim() != 2:
@@ -803,6 +809,7 @@ def layer_norm_forward(x, weight, bias, eps: float, want_stats: bool):
     xid = dtype_id(x, "x")
     device = _device_of(x, weight=weight, bias=bias)
     N, E = x.shape
+    _sizes32(E)
     wid, wp, bp = xid, None, None
     if weight is not None:
         wid, wp = dtype_id(weight, "weight"), weight.data_ptr()
@@ -855,6 +862,7 @@ def distill_topk_forward(logits, top_values, top_indices, top_lse, temperature: 
     device = _device_of(logits, top_values=top_values, top_indices=top_indices, top_lse=top_lse)
     rows, V = logits.shape
     k = top_indices.shape[1]
+    _sizes32(V, k)
     if top_values.shape != (rows, k) or top_indices.shape != (rows, k) or (top_lse is not None and top_lse.shape != (rows,)):
         raise NativeError(f"distill_topk: {rows} rows of logits, top_values {tuple(top_values.shape)}, top_indices {tuple(top_indices.shape)}"
                           + (f", top_lse {tuple(top_lse.shape)}" if top_lse is not None else ""))
@@ -895,6 +903,7 @@ def mx4_quantize(x: torch.Tensor):
     xid = dtype_id(x, "x")
     device = _device_of(x)
     rows, K = x.shape
+    _sizes32(K)
     nb = (K + 31) // 32
     codes = torch.empty((rows, nb * 16), dtype=torch.uint8, device=x.device)
     scales = torch.empty((rows, nb), dtype=torch.uint8, device=x.device)
@@ -919,6 +928,7 @@ def mx4_dequantize(codes, scales, K: int, dtype) -> torch.Tensor:
 def _mx4_operand(codes, scales, K: int, what: str) -> int:
     device = _device_of(codes, scales=scales)
     _dense(codes, torch.uint8, "codes"); _dense(scales, torch.uint8, "scales")
+    _sizes32(K, codes.shape[0])
     nb = (K + 31) // 32
     if K < 1 or codes.dim() != 2 or codes.shape != (scales.shape[0], nb * 16) or scales.shape != (codes.shape[0], nb):
         raise NativeError(f"{what}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not a 4-bit matrix of {K} columns")
@@ -941,6 +951,7 @@ def mx4_linear(x, codes, scales, bias=None) -> torch.Tensor:
     """x (M, K) @ W.T + bias for a 4-bit weight W (N, K); the result has x's type."""
     xid = dtype_id(x, "x")
     M, K = x.shape
+    _sizes32(M)
     device = _mx4_operand(codes, scales, K, "mx4_linear")
     _device_of(x, codes=codes)
     N = codes.shape[0]
@@ -959,6 +970,7 @@ def mx4_linear_dgrad(dy, codes, scales, K: int) -> torch.Tensor:
     device = _mx4_operand(codes, scales, K, "mx4_linear_dgrad")
     _device_of(dy, codes=codes)
     M, N = dy.shape
+    _sizes32(M)
     if codes.shape[0] != N:
         raise NativeError(f"mx4_linear_dgrad: gradient has {N} columns, the weight {codes.shape[0]} rows")
     dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
@@ -974,6 +986,7 @@ def mx4_bias_grad(dy, dtype) -> torch.Tensor:
     yid = dtype_id(dy, "dy")
     device = _device_of(dy)
     M, N = dy.shape
+    _sizes32(M, N)
     db = torch.empty(N, dtype=dtype, device=dy.device)
     if not M or not N:
         return db.zero_()

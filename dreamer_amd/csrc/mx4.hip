@@ -998,7 +998,7 @@ extern "C" int drm_mx4_linear_dgrad(const void* dy, int64_t lddy, int32_t dtype,
     if (int rc = mx4_check(__func__, codes, scales, N, K)) return rc;
     if (int rc = mx4_check_product(__func__, dy, lddy, dtype, N, nullptr, 0, dx, lddx, K, M)) return rc;
     if (int rc = mx4_check_tiles(__func__, M, K, K)) return rc;
-    DRM_REQUIRE(N >= 1, DRM_EINVAL, "N=%d", N);
+    DRM_REQUIRE(N >= 1 && N <= (1 << 30), DRM_EINVAL, "N=%d", N);
     if (int rc = mx4_check_workspace(__func__, workspace, workspace_bytes, drm_mx4_linear_dgrad_workspace_bytes(dtype, M, N, K))) return rc;
     hipStream_t s = (hipStream_t)stream;
     const Mx4 W{codes, scales, N, mx4_blocks(K)};

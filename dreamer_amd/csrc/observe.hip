@@ -413,6 +413,12 @@ __global__ __launch_bounds__(256) void k_observe_st_bwd(const StBwdArgs P) {
 }
 
 // defined in imagine.hip's translation unit as well; both are file-local
+// (a kernel rather than a memset: callers record this pass into graphs, where memset nodes have gone wrong on later replays)
+__global__ __launch_bounds__(256) void k_zero_o(float* __restrict__ p, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) p[i] = 0.f;
+}
+
 __global__ __launch_bounds__(256) void k_transpose_cols_o(const float* __restrict__ W, int64_t ldw, int col0, int ncols,
                                                            int nrows, float* __restrict__ out) {
     __shared__ float tile[32][33];
@@ -875,7 +881,8 @@ extern "C" int drm_observe_backward_f32(const drm_dims* dims, const drm_observe_
     }
     float* dhn[2] = {dhu + (size_t)B * D, dhu + (size_t)2 * B * D};
     const int64_t TD = (int64_t)T * D, T3D = (int64_t)T * 3 * D, T4D = (int64_t)T * 4 * D, TLK = (int64_t)T * LK;
-    DRM_HIP(hipMemsetAsync(dhn[0], 0, (size_t)B * D * sizeof(float), s));
+    k_zero_o<<<(int)(((int64_t)B * D + 255) / 256), 256, 0, s>>>(dhn[0], (int64_t)B * D);
+    DRM_LAUNCH_CHECK();
     auto stbwd = [&](int t, const float* dx_next, bool skip) -> int {
         // d(post)[t] from dz = (d(x)[t+1] @ lin_z) * c[t+1] + g_z[t]
         BwdEpilogue E{};
