@@ -468,46 +468,52 @@ __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__
     // A turn (16 of the reduction) fetches the next turn's fragments beside its own matrix instructions: x from LDS, the widened
     // codes of a block that was read a turn earlier.  (y: a lane half holds 16 codes in a row, eight per turn; dx: in order.)
     struct Turn { bf16x8 a, v[P][2]; };
+    uint32_t sw = 0u;
+    uint2 q[2];
+    Turn f[2];
+    const int wr = wn + l32;
+    auto codes = [&](const Stage& st, int b) {
+        if constexpr (!GRAD) {
+            if (b == 0) sw = st.sw[wr];
+            q[b & 1] = *reinterpret_cast<const uint2*>(st.w + wr * NB * 16 + mx4_code_slot<NB>(wr, b) * 16 + half * 8);
+        }
+    };
+    auto fetch = [&](const Stage& st, int t) {
+        const int b = t >> 1, c = GRAD ? t * 2 + half : b * 4 + half * 2 + (t & 1);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int r = wm + j * 32 + l32;
+                f[t & 1].v[p][j] = *reinterpret_cast<const bf16x8*>(st.x[p] + r * BK * 2 + mx4_chunk<CH>(r, c) * 16);
+            }
+        if constexpr (GRAD) f[t & 1].a = *reinterpret_cast<const bf16x8*>(st.w + wr * BK * 2 + mx4_chunk_t<CH>(wr, c) * 16);
+        else f[t & 1].a = mx4_bf16x8((t & 1) == 0 ? q[b & 1].x : q[b & 1].y, mx4_scale((sw >> (8 * b)) & 255u));
+    };
+    auto multiply = [&](int t) {
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                acc[0][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[t & 1].a, f[t & 1].v[p][j], acc[0][j], 0, 0, 0);
+        // one matrix instruction, then the LDS reads and conversions of the next turn that fit beside it
+#pragma unroll
+        for (int k = 0; k < 2 * P; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
     auto compute = [&](const Stage& st) {
-        uint32_t sw = 0u;
-        uint2 q[2];
-        Turn f[2];
-        const int wr = wn + l32;
-        if constexpr (!GRAD) sw = st.sw[wr];
-        auto codes = [&](int b) {
-            if constexpr (!GRAD) q[b & 1] = *reinterpret_cast<const uint2*>(st.w + wr * NB * 16 + mx4_code_slot<NB>(wr, b) * 16 + half * 8);
-        };
-        auto fetch = [&](int t) {
-            const int b = t >> 1, c = GRAD ? t * 2 + half : b * 4 + half * 2 + (t & 1);
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int r = wm + j * 32 + l32;
-                    f[t & 1].v[p][j] = *reinterpret_cast<const bf16x8*>(st.x[p] + r * BK * 2 + mx4_chunk<CH>(r, c) * 16);
-                }
-            if constexpr (GRAD) f[t & 1].a = *reinterpret_cast<const bf16x8*>(st.w + wr * BK * 2 + mx4_chunk_t<CH>(wr, c) * 16);
-            else f[t & 1].a = mx4_bf16x8((t & 1) == 0 ? q[b & 1].x : q[b & 1].y, mx4_scale((sw >> (8 * b)) & 255u));
-        };
-        codes(0);
-        fetch(0);
+        codes(st, 0);
+        fetch(st, 0);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < 2 * NB; ++t) {
-            if ((t & 1) == 0 && t / 2 + 1 < NB) codes(t / 2 + 1);
-            if (t + 1 < 2 * NB) fetch(t + 1);
-#pragma unroll
-            for (int p = P - 1; p >= 0; --p)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    acc[0][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[t & 1].a, f[t & 1].v[p][j], acc[0][j], 0, 0, 0);
-#pragma unroll
-            for (int k = 0; k < 2 * P; ++k) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
+            if ((t & 1) == 0 && t / 2 + 1 < NB) codes(st, t / 2 + 1);
+            if (t + 1 < 2 * NB) fetch(st, t + 1);
+            multiply(t);
         }
     };
     Held h;
@@ -523,9 +529,10 @@ __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__
     const int steps = (max(whole - begin, 0) + BK - 1) / BK;
     if constexpr (RING) {
         // Three stages, filled by direct loads only (rows of whole steps of blocks: every row's four scale bytes of a step are an
-        // aligned dword).  Stage i's loads are issued two steps ahead.  Before it is used, every wave waits until no more than the next
-        // stage's loads are under way (fences keep the loads of a stage together) and meets the others; behind that barrier the
-        // stage of the step before is free for new loads.
+        // aligned dword).  The waves meet before the last turn of a step, when all they need of its stage has been read: behind that
+        // barrier the stage takes the loads of the step three ahead, the next one -- which every wave has waited for, leaving no more
+        // than one later stage's loads under way (fences keep the loads of a stage together) -- gives its first fragments while
+        // the last turn runs.
         constexpr int AHEAD = 128 * CH / TILE_THREADS + NB * 2 / TILE_WAVES + 1;
         static_assert(NB * 2 % TILE_WAVES == 0, "every wave brings as much");
         auto issue = [&](Stage& st, int k0) {
@@ -537,23 +544,40 @@ __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__
             load(st, k0, h, false);
             asm volatile("" ::: "memory");
         };
-        auto turn = [&](Stage& st, int k0, Stage& after) {
-            __builtin_amdgcn_s_waitcnt((AHEAD & 15) | (AHEAD >> 4) << 14 | 0x0070);      // vmcnt(AHEAD), lgkmcnt(0)
+        auto meet = [&](auto loads) {
+            constexpr int L = decltype(loads)::value;
+            __builtin_amdgcn_s_waitcnt((L & 15) | (L >> 4) << 14 | 0x0070);      // vmcnt(L), lgkmcnt(0)
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_barrier();
-            issue(after, k0 + 2 * BK);
-            compute(st);
+            asm volatile("" ::: "memory");
+        };
+        auto step = [&](Stage& st, const Stage& next, int k0) {
+#pragma unroll
+            for (int t = 0; t + 1 < 2 * NB; ++t) {
+                if ((t & 1) == 0 && t / 2 + 1 < NB) codes(st, t / 2 + 1);
+                fetch(st, t + 1);
+                multiply(t);
+            }
+            meet(std::integral_constant<int, AHEAD>{});
+            issue(st, k0 + 3 * BK);
+            codes(next, 0);
+            fetch(next, 0);
+            multiply(2 * NB - 1);
         };
         issue(s0, begin);
         issue(s1, begin + BK);
+        issue(s2, begin + 2 * BK);
+        meet(std::integral_constant<int, 2 * AHEAD>{});
+        codes(s0, 0);
+        fetch(s0, 0);
         int k0 = begin;
         for (int p = 0; p < steps / 3; ++p, k0 += 3 * BK) {
-            turn(s0, k0, s2);
-            turn(s1, k0 + BK, s0);
-            turn(s2, k0 + 2 * BK, s1);
+            step(s0, s1, k0);
+            step(s1, s2, k0 + BK);
+            step(s2, s0, k0 + 2 * BK);
         }
-        if (steps % 3 > 0) turn(s0, k0, s2);
-        if (steps % 3 > 1) turn(s1, k0 + BK, s0);
+        if (steps % 3 > 0) step(s0, s1, k0);
+        if (steps % 3 > 1) step(s1, s2, k0 + BK);
     } else if (steps > 0) {
         load(s0, begin, h, false);
         put(s0, begin, h, false);
