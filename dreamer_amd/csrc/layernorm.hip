@@ -67,13 +67,15 @@ struct RowPart {
     }
     // f(value, c, i) for every element; one that is not its slot's own (see raw_slot) comes as `fill`
     template <typename F>
+    __device__ __forceinline__ void each_of(int c, int t, int E, float fill, F&& f) const {
+        const int at = (c * TPB + t) * VEC, foreign = at - (int)slot_at<T>(at, E);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f(i >= foreign ? (float)s[c].v[i] : fill, c, i);
+    }
+    template <typename F>
     __device__ __forceinline__ void each(int t, int E, float fill, F&& f) const {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int at = (c * TPB + t) * VEC, foreign = at - (int)slot_at<T>(at, E);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) f(i >= foreign ? (float)s[c].v[i] : fill, c, i);
-        }
+        for (int c = 0; c < CH; ++c) each_of(c, t, E, fill, f);
     }
     // store f(value, c, i); a slot that was moved back writes some of its neighbour's results once more, computed like the others
     template <typename F>
@@ -162,8 +164,87 @@ __global__ __launch_bounds__(TPB <= 64 ? 256 : TPB) void k_norm_fwd(const T* __r
     }
 }
 
-// Rows too long for registers (three walks over the row; the second and third find it in the caches unless it is longer than
-// those) and rows shorter than a slot.  One workgroup per row, four slots under way per thread.
+// Rows shorter than a slot: a row per thread, its elements one by one (a wave's rows lie side by side, so that their lines are
+// read once).
+template <typename T>
+__global__ __launch_bounds__(256) void k_norm_fwd_narrow(const T* __restrict__ x, int64_t ldx, const void* w, const void* b, int wtype,
+                                                         T* __restrict__ y, int64_t ldy, float* __restrict__ mean,
+                                                         float* __restrict__ rstd, int64_t N, int E, float eps) {
+    constexpr int M = Elem<T>::VEC - 1;
+    const float inv = 1.f / (float)E;
+    float wv[M], bv[M], v[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        wv[i] = i < E && w != nullptr ? load_elem(w, wtype, i) : 1.f;
+        bv[i] = i < E && b != nullptr ? load_elem(b, wtype, i) : 0.f;
+    }
+    for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < N; n += (int64_t)gridDim.x * 256) {
+        float sum = 0.f, q = 0.f;
+#pragma unroll
+        for (int i = 0; i < M; ++i) { v[i] = i < E ? (float)x[n * ldx + i] : 0.f; sum += v[i]; }
+        const float m = sum * inv;
+#pragma unroll
+        for (int i = 0; i < M; ++i) q += i < E ? (v[i] - m) * (v[i] - m) : 0.f;
+        const float r = 1.f / sqrtf(q * inv + eps);
+        if (mean != nullptr) { mean[n] = m; rstd[n] = r; }
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+            if (i < E) y[n * ldy + i] = (T)fmaf((v[i] - m) * r, wv[i], bv[i]);
+    }
+}
+// backward: a workgroup's column sums by lanes, then wave after wave (see k_norm_bwd for `partials`)
+template <typename T>
+__global__ __launch_bounds__(256) void k_norm_bwd_narrow(const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy, int64_t lddy,
+                                                         const void* w, int wtype, const float* __restrict__ mean,
+                                                         const float* __restrict__ rstd, T* __restrict__ dx,
+                                                         float* __restrict__ partials, int64_t N, int E) {
+    constexpr int M = Elem<T>::VEC - 1;
+    __shared__ float s_wave[4][2 * M];
+    const float inv = 1.f / (float)E;
+    float wv[M], aw[M], ab[M], d[M], h[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        wv[i] = i < E && w != nullptr ? load_elem(w, wtype, i) : 1.f;
+        aw[i] = 0.f;
+        ab[i] = 0.f;
+    }
+    for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < N; n += (int64_t)gridDim.x * 256) {
+        const float m = mean[n], r = rstd[n];
+        float s = 0.f, q = 0.f;
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            d[i] = i < E ? (float)dy[n * lddy + i] : 0.f;
+            h[i] = i < E ? ((float)x[n * ldx + i] - m) * r : 0.f;
+            aw[i] = fmaf(d[i], h[i], aw[i]);
+            ab[i] += d[i];
+            s = fmaf(d[i], wv[i], s);
+            q = fmaf(d[i] * wv[i], h[i], q);
+        }
+        if (dx == nullptr) continue;
+        s *= inv; q *= inv;
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+            if (i < E) dx[n * (int64_t)E + i] = (T)(r * (fmaf(d[i], wv[i], -s) - h[i] * q));
+    }
+    if (partials == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        aw[i] = group_sum<64>(aw[i]);
+        ab[i] = group_sum<64>(ab[i]);
+    }
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int i = 0; i < M; ++i) { s_wave[threadIdx.x >> 6][i] = aw[i]; s_wave[threadIdx.x >> 6][M + i] = ab[i]; }
+    }
+    __syncthreads();
+    const int i = threadIdx.x % M, half = threadIdx.x / M;
+    if (half < 2 && i < E)
+        partials[((int64_t)blockIdx.x * 2 + half) * E + i] =
+            (s_wave[0][half * M + i] + s_wave[1][half * M + i]) + (s_wave[2][half * M + i] + s_wave[3][half * M + i]);
+}
+
+// Rows too long for registers: three walks over the row (the second and third find it in the caches unless it is longer than
+// those).  One workgroup per row, four slots under way per thread.
 template <typename T, int TPB>
 __global__ __launch_bounds__(TPB) void k_norm_fwd_long(const T* __restrict__ x, int64_t ldx, const void* w, const void* b, int wtype,
                                                        T* __restrict__ y, int64_t ldy, float* __restrict__ mean,
@@ -229,17 +310,38 @@ __global__ __launch_bounds__(TPB <= 64 ? 256 : TPB, 4) void k_norm_bwd(const T* 
                                                                     T* __restrict__ dx, float* __restrict__ partials, int64_t N,
                                                                     int E) {
     constexpr int VEC = Elem<T>::VEC, RPB = TPB <= 64 ? 256 / TPB : 1;
-    constexpr bool KEEP = CH * VEC <= 8, AHEAD = KEEP;            // (sixteen elements at 1024 threads: 128 registers each)
+    // sixteen elements at 1024 threads, 128 registers each: the weight is read again for every row, and the column sums stay in
+    // LDS, each thread's its own (2 x 16 KiB of it moved per 6 KiB of a bf16 row: a fifth of the row's time)
+    constexpr bool KEEP = CH * VEC <= 8, AHEAD = KEEP || sizeof(T) == 2;      // (fp32: no registers left for the next row's)
     using Part = RowPart<T, TPB, CH>;
     __shared__ float s_buf[2][TPB <= 64 ? 1 : TPB / 64][2];
     __shared__ float s_cols[TPB <= 64 ? TPB * CH * VEC : 1];
+    __shared__ f32x4 s_sums[KEEP ? 1 : CH * VEC / 4 * 2][KEEP ? 1 : TPB];
     const int t = threadIdx.x % TPB;
     float wv[CH][VEC], aw[CH][VEC], ab[CH][VEC];
+    auto sums_from = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            aw[c][i] = s_sums[(c * VEC + i) / 4 * 2][t][i & 3];
+            ab[c][i] = s_sums[(c * VEC + i) / 4 * 2 + 1][t][i & 3];
+        }
+    };
+    auto sums_to = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) {
+            s_sums[(c * VEC + i) / 4 * 2][t] = f32x4{aw[c][i], aw[c][i + 1], aw[c][i + 2], aw[c][i + 3]};
+            s_sums[(c * VEC + i) / 4 * 2 + 1][t] = f32x4{ab[c][i], ab[c][i + 1], ab[c][i + 2], ab[c][i + 3]};
+        }
+    };
     if constexpr (KEEP) load_columns<T, TPB, CH>(w, wtype, 1.f, t, E, wv);
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) { aw[c][i] = 0.f; ab[c][i] = 0.f; }
+    if constexpr (!KEEP) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) sums_to(c);
+    }
     const float inv = 1.f / (float)E;
     const int64_t step = (int64_t)gridDim.x * RPB;
     Part nx, nd;
@@ -262,14 +364,19 @@ __global__ __launch_bounds__(TPB <= 64 ? 256 : TPB, 4) void k_norm_bwd(const T* 
         if constexpr (AHEAD) fetch(n + step);
         if constexpr (!KEEP) load_columns<T, TPB, CH>(w, wtype, 1.f, t, E, wv);
         float s = 0.f, q = 0.f;
-        pd.each(t, E, 0.f, [&](float d, int c, int i) {
-            if (TPB <= 64 && !live) d = 0.f;
-            const float h = ((float)px.s[c].v[i] - m) * r, gw = d * wv[c][i];
-            aw[c][i] = fmaf(d, h, aw[c][i]);
-            ab[c][i] += d;
-            s += gw;
-            q = fmaf(gw, h, q);
-        });
+#pragma unroll
+        for (int k = 0; k < CH; ++k) {
+            if constexpr (!KEEP) sums_from(k);
+            pd.each_of(k, t, E, 0.f, [&](float d, int c, int i) {
+                if (TPB <= 64 && !live) d = 0.f;
+                const float h = ((float)px.s[c].v[i] - m) * r, gw = d * wv[c][i];
+                aw[c][i] = fmaf(d, h, aw[c][i]);
+                ab[c][i] += d;
+                s += gw;
+                q = fmaf(gw, h, q);
+            });
+            if constexpr (!KEEP) sums_to(k);
+        }
         row_sum2<TPB>(s, q, s_buf[flip]);
         if (dx != nullptr && live) {
             s *= inv; q *= inv;
@@ -314,7 +421,8 @@ __global__ __launch_bounds__(TPB <= 64 ? 256 : TPB, 4) void k_norm_bwd(const T* 
             }
     } else {
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
+        for (int c = 0; c < CH; ++c) {
+            if constexpr (!KEEP) sums_from(c);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const int at = (c * TPB + t) * VEC;
@@ -323,23 +431,24 @@ __global__ __launch_bounds__(TPB <= 64 ? 256 : TPB, 4) void k_norm_bwd(const T* 
                     pw[E + slot_at<T>(at, E) + i] = ab[c][i];
                 }
             }
+        }
     }
 }
 
-// the same rows backward: the two row means first ...
+// the long rows backward: the two row means first ...
 template <typename T, int TPB>
 __global__ __launch_bounds__(TPB) void k_norm_bwd_sums(const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy, int64_t lddy,
                                                         const void* w, int wtype, const float* __restrict__ mean,
                                                         const float* __restrict__ rstd, float* __restrict__ sums, int64_t N, int E) {
-    constexpr int VEC = Elem<T>::VEC;
+    constexpr int VEC = Elem<T>::VEC, U = 2, STEP = TPB * VEC;
     __shared__ float s_buf[2][TPB / 64][2];
+    const int64_t bulk = (int64_t)E / (U * STEP) * (U * STEP);       // whole slots of every thread
     int flip = 0;
     for (int64_t n = blockIdx.x; n < N; n += gridDim.x, flip ^= 1) {
         const float m = mean[n], r = rstd[n];
+        const T *rx = x + n * ldx, *rg = dy + n * lddy;
         float xv[VEC], g[VEC], s = 0.f, q = 0.f;
-        for (int64_t e = (int64_t)threadIdx.x * VEC; e < E; e += TPB * VEC) {
-            load_slot(x + n * ldx, e, E, m, xv);
-            load_slot(dy + n * lddy, e, E, 0.f, g);
+        auto one = [&](int64_t e) {
             float ps = 0.f, pq = 0.f;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
@@ -348,6 +457,25 @@ __global__ __launch_bounds__(TPB) void k_norm_bwd_sums(const T* __restrict__ x, 
                 pq = fmaf(gw, (xv[i] - m) * r, pq);
             }
             s += ps; q += pq;
+        };
+        for (int64_t e = (int64_t)threadIdx.x * VEC; e < bulk; e += U * STEP) {
+            Slot<T> sx[U], sg[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                sx[u] = *reinterpret_cast<const Slot<T>*>(rx + e + u * STEP);
+                sg[u] = *reinterpret_cast<const Slot<T>*>(rg + e + u * STEP);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) { xv[i] = (float)sx[u].v[i]; g[i] = (float)sg[u].v[i]; }
+                one(e + u * STEP);
+            }
+        }
+        for (int64_t e = bulk + (int64_t)threadIdx.x * VEC; e < E; e += STEP) {
+            load_slot(rx, e, E, m, xv);
+            load_slot(rg, e, E, 0.f, g);
+            one(e);
         }
         row_sum2<TPB>(s, q, s_buf[flip]);
         if (threadIdx.x == 0) { sums[2 * n] = s / (float)E; sums[2 * n + 1] = q / (float)E; }
@@ -369,11 +497,8 @@ __global__ __launch_bounds__(256) void k_norm_bwd_cols(const T* __restrict__ x, 
         aw[i] = 0.f;
         ab[i] = 0.f;
     }
-    for (int64_t n = blockIdx.y; n < N; n += gridDim.y) {
+    auto one = [&](int64_t n, const float (&xv)[VEC], float (&g)[VEC]) {
         const float m = mean[n], r = rstd[n];
-        float xv[VEC], g[VEC];
-        load_slot(x + n * ldx, e, E, m, xv);
-        load_slot(dy + n * lddy, e, E, 0.f, g);
         const float s = sums != nullptr ? sums[2 * n] : 0.f, q = sums != nullptr ? sums[2 * n + 1] : 0.f;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
@@ -383,6 +508,31 @@ __global__ __launch_bounds__(256) void k_norm_bwd_cols(const T* __restrict__ x, 
             g[i] = r * (g[i] * wv[i] - fmaf(h, q, s));
         }
         if (dx != nullptr) store_slot(dx + n * (int64_t)E, e, E, g);
+    };
+    float xv[VEC], g[VEC];
+    int64_t n = blockIdx.y;
+    if (e + VEC <= E) {
+        // whole slots: four rows under way
+        constexpr int U = 4;
+        for (; n + (U - 1) * (int64_t)gridDim.y < N; n += U * (int64_t)gridDim.y) {
+            Slot<T> rx[U], rg[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                rx[u] = *reinterpret_cast<const Slot<T>*>(x + (n + u * (int64_t)gridDim.y) * ldx + e);
+                rg[u] = *reinterpret_cast<const Slot<T>*>(dy + (n + u * (int64_t)gridDim.y) * lddy + e);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) { xv[i] = (float)rx[u].v[i]; g[i] = (float)rg[u].v[i]; }
+                one(n + u * (int64_t)gridDim.y, xv, g);
+            }
+        }
+    }
+    for (; n < N; n += gridDim.y) {
+        load_slot(x + n * ldx, e, E, mean[n], xv);
+        load_slot(dy + n * lddy, e, E, 0.f, g);
+        one(n, xv, g);
     }
     if (partials != nullptr) {
         float* pw = partials + (int64_t)blockIdx.y * 2 * E;
@@ -428,13 +578,13 @@ __global__ __launch_bounds__(1024) void k_norm_cols(const float* __restrict__ pa
 // sums: 80 to 100 registers, four to five waves per SIMD) up to 8192, sixteen at 1024 threads; forward sixteen, 32 at 1024 threads.
 constexpr int NORM_MAX_E = 1024 * 16, NORM_MAX_E_FWD = 1024 * 32;
 template <typename T>
-static inline bool norm_short(int E) { return E < Elem<T>::VEC; }
-static inline bool norm_long_bwd(int E, int x_dtype) { return E > NORM_MAX_E || E < (x_dtype == DRM_F32 ? 4 : 8); }
+static inline bool norm_narrow(int E) { return E < Elem<T>::VEC; }
 // workgroups that walk the rows backward (about sixteen waves a CU): each leaves 2 E column sums
 static inline int norm_slices(int64_t N, int E, int x_dtype) {
     if (N < 1) return 1;
-    if (norm_long_bwd(E, x_dtype)) return (int)(N < 64 ? N : 64);
     const int vec = x_dtype == DRM_F32 ? 4 : 8;
+    if (E > NORM_MAX_E) return (int)(N < 64 ? N : 64);
+    if (E < vec) return (int)std::min<int64_t>((N + 255) / 256, 1024);
     const int64_t rpb = E <= 8 * vec ? 32 : E <= 16 * vec ? 16 : E <= 32 * vec ? 8 : E <= 512 ? 4 : 1, groups = (N + rpb - 1) / rpb;
     const int64_t cap = E <= 512 ? 1024 : E <= 1024 ? 2048 : E <= 2048 ? 1024 : E <= 4096 ? 512 : 256;
     return (int)(groups < cap ? groups : cap);
@@ -488,11 +638,10 @@ extern "C" int drm_layer_norm_forward(const void* x, int64_t ldx, int32_t x_dtyp
     ProfScope ps(PC_ELEMENTWISE, s, 8 * n, 2 * n * elem_bytes(x_dtype));
     return with_elem(x_dtype, [&](auto tag) -> int {
         using T = decltype(tag);
-        const int long_grid = (int)(N < 4096 ? N : 4096);
-        if (norm_short<T>(E)) {
-            k_norm_fwd_long<T, 64><<<long_grid, 64, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
+        if (norm_narrow<T>(E)) {
+            k_norm_fwd_narrow<T><<<(int)std::min<int64_t>((N + 255) / 256, 2048), 256, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
         } else if (E > NORM_MAX_E_FWD) {
-            k_norm_fwd_long<T, 1024><<<long_grid, 1024, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
+            k_norm_fwd_long<T, 1024><<<(int)(N < 4096 ? N : 4096), 1024, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
         } else if (E > NORM_MAX_E) {
             k_norm_fwd<T, 1024, 32 / Elem<T>::VEC, false><<<(int)(N < 512 ? N : 512), 1024, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
         } else {
@@ -513,7 +662,7 @@ extern "C" size_t drm_layer_norm_workspace_bytes(int64_t N, int32_t E) {
     if (N < 0 || E < 1) return 0;
     size_t need = 0;
     for (int t : {DRM_F32, DRM_BF16}) {
-        const size_t sums = norm_long_bwd(E, t) ? (size_t)N * 2 * sizeof(float) : 0;
+        const size_t sums = E > NORM_MAX_E ? (size_t)N * 2 * sizeof(float) : 0;
         need = std::max(need, sums + (size_t)norm_slices(N, E, t) * 2 * E * sizeof(float));
     }
     return need;
@@ -537,18 +686,18 @@ extern "C" int drm_layer_norm_backward(const void* x, int64_t ldx, const void* d
     DRM_REQUIRE(workspace && workspace_bytes >= drm_layer_norm_workspace_bytes(N, E), DRM_EINVAL, "workspace of %zu bytes, %zu needed",
                 workspace ? workspace_bytes : (size_t)0, drm_layer_norm_workspace_bytes(N, E));
     const int slices = norm_slices(N, E, x_dtype);
-    const bool walk = norm_long_bwd(E, x_dtype);
+    const bool walk = E > NORM_MAX_E;
     const double n = (double)N * E;
     ProfScope ps(PC_ELEMENTWISE, s, 17 * n, 3 * n * elem_bytes(x_dtype));
     float* sums = (float*)workspace;
     float* part = !cols ? nullptr : walk ? sums + 2 * N : sums;
     const int rc = with_elem(x_dtype, [&](auto tag) -> int {
         using T = decltype(tag);
-        if (walk) {
+        if (norm_narrow<T>(E)) {
+            k_norm_bwd_narrow<T><<<slices, 256, 0, s>>>((const T*)x, ldx, (const T*)dy, lddy, w, w_dtype, mean, rstd, (T*)dx, part, N, E);
+        } else if (walk) {
             if (dx != nullptr) {
-                const int grid = (int)(N < 4096 ? N : 4096);
-                if (norm_short<T>(E)) k_norm_bwd_sums<T, 64><<<grid, 64, 0, s>>>((const T*)x, ldx, (const T*)dy, lddy, w, w_dtype, mean, rstd, sums, N, E);
-                else k_norm_bwd_sums<T, 1024><<<grid, 1024, 0, s>>>((const T*)x, ldx, (const T*)dy, lddy, w, w_dtype, mean, rstd, sums, N, E);
+                k_norm_bwd_sums<T, 1024><<<(int)(N < 4096 ? N : 4096), 1024, 0, s>>>((const T*)x, ldx, (const T*)dy, lddy, w, w_dtype, mean, rstd, sums, N, E);
                 DRM_LAUNCH_CHECK();
             }
             constexpr int STRIP = 256 * Elem<T>::VEC;

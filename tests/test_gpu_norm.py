@@ -90,6 +90,12 @@ def test_many_rows_reduce_into_the_weight_gradient(rows, E):
     assert all(torch.equal(s, t) for s, t in zip(a, b))              # no order of workgroups in the results
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,E,stride", [(70000, 3, 3), (3000, 7, 9), (257, 1, 5), (64, 4, 4), (40, 17000, 17008), (300, 9001, 9001)])
+def test_narrow_rows_and_long_ones(rows, E, stride, dtype):
+    _check(*_inputs(rows, E, dtype, F32, stride=stride))
+
+
 def test_rows_far_from_zero_keep_their_digits():
     x, w, b, dy = _inputs(9, 777, F32, F32, offset=1000.0)
     _check(x, w, b, dy)
