@@ -121,6 +121,27 @@ __device__ __forceinline__ void load_columns(const void* p, int type, float abse
     }
 }
 
+// the same for one slot: whole ones by wide loads
+template <typename T>
+__device__ __forceinline__ void load_column(const void* p, int type, float absent, int64_t e, int E, float (&v)[Elem<T>::VEC]) {
+    constexpr int VEC = Elem<T>::VEC;
+    if (p == nullptr || e + VEC > E) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = p != nullptr ? load_elem(p, type, min(e + i, (int64_t)E - 1)) : absent;
+    } else if (type == DRM_F32) {
+#pragma unroll
+        for (int h = 0; h < VEC; h += 4) {
+            const Slot<float> s = *reinterpret_cast<const Slot<float>*>(reinterpret_cast<const float*>(p) + e + h);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[h + i] = s.v[i];
+        }
+    } else {
+        const Slot<T> s = *reinterpret_cast<const Slot<T>*>(reinterpret_cast<const T*>(p) + e);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = (float)s.v[i];
+    }
+}
+
 // TPB threads per row: up to 64 one or several rows per wave (256 threads a workgroup), above one workgroup per row.
 // KEEP: the weight and the bias stay in registers from row to row; without, they are read again (rows of more than 16 elements
 // a thread)
@@ -291,12 +312,11 @@ __global__ __launch_bounds__(TPB) void k_norm_fwd_long(const T* __restrict__ x, 
         const float r = 1.f / sqrtf(row_sum<TPB>(q, s_buf[1]) * inv + eps);
         if (threadIdx.x == 0 && mean != nullptr) { mean[n] = m; rstd[n] = r; }
         walk([&](const float (&v)[VEC], int, int64_t e) {
-            float o[VEC];
+            float o[VEC], wv[VEC], bv[VEC];
+            load_column<T>(w, wtype, 1.f, e, E, wv);
+            load_column<T>(b, wtype, 0.f, e, E, bv);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const int64_t k = min(e + i, (int64_t)E - 1);
-                o[i] = fmaf((v[i] - m) * r, w != nullptr ? load_elem(w, wtype, k) : 1.f, b != nullptr ? load_elem(b, wtype, k) : 0.f);
-            }
+            for (int i = 0; i < VEC; ++i) o[i] = fmaf((v[i] - m) * r, wv[i], bv[i]);
             store_slot(y + n * ldy, e, E, o);
         });
     }
@@ -449,10 +469,11 @@ __global__ __launch_bounds__(TPB) void k_norm_bwd_sums(const T* __restrict__ x, 
         const T *rx = x + n * ldx, *rg = dy + n * lddy;
         float xv[VEC], g[VEC], s = 0.f, q = 0.f;
         auto one = [&](int64_t e) {
-            float ps = 0.f, pq = 0.f;
+            float ps = 0.f, pq = 0.f, wv[VEC];
+            load_column<T>(w, wtype, 1.f, e, E, wv);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const float gw = g[i] * (w != nullptr ? load_elem(w, wtype, min(e + i, (int64_t)E - 1)) : 1.f);
+                const float gw = g[i] * wv[i];
                 ps += gw;
                 pq = fmaf(gw, (xv[i] - m) * r, pq);
             }
@@ -576,7 +597,9 @@ __global__ __launch_bounds__(1024) void k_norm_cols(const float* __restrict__ pa
 // ---- host side -------------------------------------------------------------------------------------------------------
 // Threads per row by the row's length.  Backward holds eight elements a thread (x, dy, the next row's, weight, two running column
 // sums: 80 to 100 registers, four to five waves per SIMD) up to 8192, sixteen at 1024 threads; forward sixteen, 32 at 1024 threads.
-constexpr int NORM_MAX_E = 1024 * 16, NORM_MAX_E_FWD = 1024 * 32;
+constexpr int NORM_MAX_E = 1024 * 16;
+template <typename T>
+static constexpr int norm_max_fwd() { return sizeof(T) == 2 ? 2 * NORM_MAX_E : NORM_MAX_E; }
 template <typename T>
 static inline bool norm_narrow(int E) { return E < Elem<T>::VEC; }
 // workgroups that walk the rows backward (about sixteen waves a CU): each leaves 2 E column sums
@@ -640,10 +663,11 @@ extern "C" int drm_layer_norm_forward(const void* x, int64_t ldx, int32_t x_dtyp
         using T = decltype(tag);
         if (norm_narrow<T>(E)) {
             k_norm_fwd_narrow<T><<<(int)std::min<int64_t>((N + 255) / 256, 2048), 256, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
-        } else if (E > NORM_MAX_E_FWD) {
-            k_norm_fwd_long<T, 1024><<<(int)(N < 4096 ? N : 4096), 1024, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
+        } else if (E > norm_max_fwd<T>()) {
+            k_norm_fwd_long<T, 512><<<(int)(N < 4096 ? N : 4096), 512, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
         } else if (E > NORM_MAX_E) {
-            k_norm_fwd<T, 1024, 32 / Elem<T>::VEC, false><<<(int)(N < 512 ? N : 512), 1024, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
+            if constexpr (sizeof(T) == 2)
+                k_norm_fwd<T, 1024, 4, false><<<(int)(N < 512 ? N : 512), 1024, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
         } else {
             norm_variant<T, false>(E, [&](auto tpb, auto ch) {
                 constexpr int TPB = decltype(tpb)::value, CH = decltype(ch)::value, RPB = TPB <= 64 ? 256 / TPB : 1;
