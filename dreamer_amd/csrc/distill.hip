@@ -373,7 +373,7 @@ extern "C" int drm_distill_topk_forward(const void* logits, int64_t ld_logits, i
     return with_elem(dtype, [&](auto tag) -> int {
         using T = decltype(tag);
         const int grid = (int)(rows * A.segs);
-        if (V <= 2048) k_distill_fwd<T, 64><<<grid, 64, 0, s>>>(A, c);
+        if (V <= 4096) k_distill_fwd<T, 64><<<grid, 64, 0, s>>>(A, c);
         else k_distill_fwd<T, 256><<<grid, 256, 0, s>>>(A, c);
         DRM_LAUNCH_CHECK();
         if (A.segs > 1) {

@@ -8,7 +8,7 @@
 // read once and the variance is taken about the mean.  Workgroups walk over rows: the weight and the bias stay in registers
 // for all of them, and so do the column sums of the backward pass, which go to `partials` once per workgroup and are added
 // there in a fixed order (no atomics: results do not depend on the order in which workgroups run).
-#include "elem.hpp"
+#include "colsum.hpp"
 
 #include <algorithm>
 #include <type_traits>
@@ -333,6 +333,7 @@ __global__ __launch_bounds__(TPB <= 64 ? 256 : TPB, 4) void k_norm_bwd(const T* 
     // sixteen elements at 1024 threads, 128 registers each: the weight is read again for every row, and the column sums stay in
     // LDS, each thread's its own (2 x 16 KiB of it moved per 6 KiB of a bf16 row: a fifth of the row's time)
     constexpr bool KEEP = CH * VEC <= 8, AHEAD = KEEP || sizeof(T) == 2;      // (fp32: no registers left for the next row's)
+    static_assert(KEEP || TPB > 64, "column sums in LDS: one row per workgroup");
     using Part = RowPart<T, TPB, CH>;
     __shared__ float s_buf[2][TPB <= 64 ? 1 : TPB / 64][2];
     __shared__ float s_cols[TPB <= 64 ? TPB * CH * VEC : 1];
@@ -563,37 +564,6 @@ __global__ __launch_bounds__(256) void k_norm_bwd_cols(const T* __restrict__ x, 
     }
 }
 
-// Column sums over the slices: 32 columns x 32 groups of slices per workgroup (the sum is short of bytes and long of latency: eight
-// loads under way per thread), groups added in order.  Column c < E: dw, else db.
-__global__ __launch_bounds__(1024) void k_norm_cols(const float* __restrict__ partials, int slices, int E, int wtype, void* dw, void* db) {
-    __shared__ float s_part[32][33];
-    const int g = threadIdx.x >> 5, l = threadIdx.x & 31;
-    const int64_t c = (int64_t)blockIdx.x * 32 + l, cols = 2 * (int64_t)E;
-    float a[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) a[u] = 0.f;
-    if (c < cols) {
-        int s = g;
-        for (; s + 7 * 32 < slices; s += 8 * 32) {
-            float v[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = partials[(int64_t)(s + u * 32) * cols + c];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) a[u] += v[u];
-        }
-        for (; s < slices; s += 32) a[0] += partials[(int64_t)s * cols + c];
-    }
-    s_part[g][l] = ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
-    __syncthreads();
-    if (g == 0 && c < cols) {
-        float v = 0.f;
-#pragma unroll
-        for (int k = 0; k < 32; ++k) v += s_part[k][l];
-        if (c < E) { if (dw != nullptr) store_elem(dw, wtype, c, v); }
-        else if (db != nullptr) store_elem(db, wtype, c - E, v);
-    }
-}
-
 // ---- host side -------------------------------------------------------------------------------------------------------
 // Threads per row by the row's length.  Backward holds eight elements a thread (x, dy, the next row's, weight, two running column
 // sums: 80 to 100 registers, four to five waves per SIMD) up to 8192, sixteen at 1024 threads; forward sixteen, 32 at 1024 threads.
@@ -609,8 +579,8 @@ static inline int norm_slices(int64_t N, int E, int x_dtype) {
     if (E > NORM_MAX_E) return (int)(N < 64 ? N : 64);
     if (E < vec) return (int)std::min<int64_t>((N + 255) / 256, 1024);
     const int64_t rpb = E <= 8 * vec ? 32 : E <= 16 * vec ? 16 : E <= 32 * vec ? 8 : E <= 512 ? 4 : 1, groups = (N + rpb - 1) / rpb;
-    const int64_t cap = E <= 512 ? 1024 : E <= 1024 ? 2048 : E <= 2048 ? 1024 : E <= 4096 ? 512 : 256;
-    return (int)(groups < cap ? groups : cap);
+    const int64_t cap = E <= 1024 ? 1024 : E <= 2048 ? 512 : 256, few = std::max<int64_t>(groups / 4, 128);
+    return (int)std::min(groups, std::min(few, cap));
 }
 
 #define DRM_NORM_CASE(TPB, CH) return f(std::integral_constant<int, TPB>{}, std::integral_constant<int, CH>{})
@@ -671,7 +641,7 @@ extern "C" int drm_layer_norm_forward(const void* x, int64_t ldx, int32_t x_dtyp
         } else {
             norm_variant<T, false>(E, [&](auto tpb, auto ch) {
                 constexpr int TPB = decltype(tpb)::value, CH = decltype(ch)::value, RPB = TPB <= 64 ? 256 / TPB : 1;
-                const int64_t groups = (N + RPB - 1) / RPB, cap = 256 * 2048 / (TPB <= 64 ? 256 : TPB);   // what the chip holds at once
+                const int64_t groups = (N + RPB - 1) / RPB, cap = 256 * 8192 / (TPB <= 64 ? 256 : TPB);   // four times what the chip holds at once
                 k_norm_fwd<T, TPB, CH, true><<<(int)(groups < cap ? groups : cap), TPB <= 64 ? 256 : TPB, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
                 return 0;
             });
@@ -699,9 +669,8 @@ extern "C" int drm_layer_norm_backward(const void* x, int64_t ldx, const void* d
     const bool cols = dw != nullptr || db != nullptr;
     DRM_REQUIRE(N >= 0 && E >= 1, DRM_EINVAL, "N=%lld E=%d", (long long)N, E);
     DRM_REQUIRE(elem_ok(x_dtype) && (w_dtype == DRM_F32 || w_dtype == x_dtype), DRM_ENOTSUP, "element types %d / %d", x_dtype, w_dtype);
-    const int cgrid = (int)((2 * (int64_t)E + 31) / 32);
     if (N == 0) {
-        if (cols) { k_norm_cols<<<cgrid, 1024, 0, s>>>(nullptr, 0, E, w_dtype, dw, db); DRM_LAUNCH_CHECK(); }
+        if (cols) { join_columns(nullptr, 0, 2 * (int64_t)E, E, w_dtype, dw, db, s); DRM_LAUNCH_CHECK(); }
         return DRM_OK;
     }
     if (int rc = norm_check(__func__, x, ldx, x_dtype, w_dtype, N, E)) return rc;
@@ -738,7 +707,7 @@ extern "C" int drm_layer_norm_backward(const void* x, int64_t ldx, const void* d
         return DRM_OK;
     });
     if (rc != DRM_OK || !cols) return rc;
-    k_norm_cols<<<cgrid, 1024, 0, s>>>(part, slices, E, w_dtype, dw, db);
+    join_columns(part, slices, 2 * (int64_t)E, E, w_dtype, dw, db, s);
     DRM_LAUNCH_CHECK();
     return DRM_OK;
 }

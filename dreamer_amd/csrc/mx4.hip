@@ -1,10 +1,10 @@
 // Microscaled 4-bit floating point: quantisation, its inverse, and the products that read 4-bit weights.
+#include "colsum.hpp"
 #include "mx4.hpp"
-
-#include <type_traits>
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 namespace drm {
 
@@ -805,18 +805,29 @@ __global__ __launch_bounds__(256) void k_mx4_join(const float* __restrict__ part
 }
 
 // ---- bias gradient: column sums of dy ----------------------------------------------------------------------------------
-// A workgroup takes 32 slots of columns x 8 rows at a time over a slice of the rows; slices meet in `part` and are added in order.
+// A workgroup takes 32 slots of columns x 8 rows at a time, four of these under way, over a slice of the rows.
 template <typename T>
 __global__ __launch_bounds__(256) void k_mx4_colsum(const T* __restrict__ dy, int64_t lddy, int M, int N, float* __restrict__ part) {
-    constexpr int VEC = Elem<T>::VEC;
+    constexpr int VEC = Elem<T>::VEC, U = 4;
     __shared__ float s_sum[8][32][VEC];
     const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
-    const int64_t c0 = ((int64_t)blockIdx.x * 32 + cl) * VEC;
+    const int64_t c0 = ((int64_t)blockIdx.x * 32 + cl) * VEC, step = (int64_t)gridDim.y * 8;
     float a[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) a[i] = 0.f;
+    int64_t m = (int64_t)blockIdx.y * 8 + rl;
+    if (c0 + VEC <= N)
+        for (; m + (U - 1) * step < M; m += U * step) {
+            Slot<T> raw[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) raw[u] = *reinterpret_cast<const Slot<T>*>(dy + (m + u * step) * lddy + c0);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) a[i] += (float)raw[u].v[i];
+        }
     if (c0 < N)
-        for (int64_t m = (int64_t)blockIdx.y * 8 + rl; m < M; m += (int64_t)gridDim.y * 8) {
+        for (; m < M; m += step) {
             float v[VEC];
             load_slot(dy + m * lddy, c0, N, 0.f, v);
 #pragma unroll
@@ -833,14 +844,11 @@ __global__ __launch_bounds__(256) void k_mx4_colsum(const T* __restrict__ dy, in
         if (c < N) part[(int64_t)blockIdx.y * N + c] = v;
     }
 }
-__global__ __launch_bounds__(256) void k_mx4_colsum_join(const float* __restrict__ part, int slices, int N, void* db, int dtype) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= N) return;
-    float v = 0.f;
-    for (int k = 0; k < slices; ++k) v += part[(int64_t)k * N + c];
-    store_elem(db, dtype, c, v);
+// about four workgroups a CU, of 32 rows at least
+static inline int mx4_colsum_slices(int M, int N) {
+    const int64_t want = std::max<int64_t>(1, 1024 / ((N + 255ll) / 256));
+    return (int)std::min<int64_t>(std::min<int64_t>(want, 256), (M + 31ll) / 32);
 }
-static inline int mx4_colsum_slices(int M) { return M <= 128 ? 1 : M <= 2048 ? (M + 127) / 128 : 16; }
 
 static inline int mx4_stream_grid(int64_t quads) { return (int)(quads < 256 * 16384ll ? (quads + 255) / 256 : 16384); }
 static inline int mx4_blocks(int K) { return K / 32 + (K % 32 != 0); }
@@ -1065,7 +1073,7 @@ extern "C" int drm_mx4_product(const uint8_t* x_codes, const uint8_t* x_scales, 
 
 extern "C" size_t drm_mx4_bias_grad_workspace_bytes(int32_t M, int32_t N) {
     if (M < 1 || N < 1) return 0;
-    return (size_t)mx4_colsum_slices(M) * N * sizeof(float);
+    return (size_t)mx4_colsum_slices(M, N) * N * sizeof(float);
 }
 
 extern "C" int drm_mx4_bias_grad(const void* dy, int64_t lddy, int32_t dtype, void* db, int32_t db_dtype, int32_t M, int32_t N,
@@ -1076,7 +1084,7 @@ extern "C" int drm_mx4_bias_grad(const void* dy, int64_t lddy, int32_t dtype, vo
     const size_t need = drm_mx4_bias_grad_workspace_bytes(M, N);
     DRM_REQUIRE(workspace && workspace_bytes >= need, DRM_EINVAL, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
     hipStream_t s = (hipStream_t)stream;
-    const int slices = mx4_colsum_slices(M);
+    const int slices = mx4_colsum_slices(M, N);
     ProfScope ps(PC_ELEMENTWISE, s, (double)M * N, (double)M * N * elem_bytes(dtype));
     const int rc = with_elem(dtype, [&](auto tag) -> int {
         using T = decltype(tag);
@@ -1086,7 +1094,7 @@ extern "C" int drm_mx4_bias_grad(const void* dy, int64_t lddy, int32_t dtype, vo
         return DRM_OK;
     });
     if (rc != DRM_OK) return rc;
-    k_mx4_colsum_join<<<(N + 255) / 256, 256, 0, s>>>((const float*)workspace, slices, N, db, db_dtype);
+    join_columns((const float*)workspace, slices, N, N, db_dtype, db, nullptr, s);
     DRM_LAUNCH_CHECK();
     return DRM_OK;
 }
