@@ -641,7 +641,7 @@ extern "C" int drm_layer_norm_forward(const void* x, int64_t ldx, int32_t x_dtyp
         } else {
             norm_variant<T, false>(E, [&](auto tpb, auto ch) {
                 constexpr int TPB = decltype(tpb)::value, CH = decltype(ch)::value, RPB = TPB <= 64 ? 256 / TPB : 1;
-                const int64_t groups = (N + RPB - 1) / RPB, cap = 256 * 8192 / (TPB <= 64 ? 256 : TPB);   // four times what the chip holds at once
+                const int64_t groups = (N + RPB - 1) / RPB, cap = TPB <= 64 ? 8192 : 256 * (TPB < 1024 ? 8192 : 2048) / TPB;
                 k_norm_fwd<T, TPB, CH, true><<<(int)(groups < cap ? groups : cap), TPB <= 64 ? 256 : TPB, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);
                 return 0;
             });
