@@ -10,7 +10,8 @@ namespace drm {
 
 // ---- quantisation -------------------------------------------------------------------------------------------------------
 // e = floor(log2(max |x|)) - 2, clamped to [-127, 127]; code = x / 2^e rounded to the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 (ties
-// to the even code), 6 beyond.  Four lanes share a block: eight elements, four code bytes each.  A stream: bound by the bytes.
+// to the even code), 6 beyond.  Four lanes share a block: eight elements, four code bytes each.  A stream: bound by the bytes
+// (12288 x 4096 bf16 20 us, 6.5 TB/s; 16384 x 8192 fp32 115 us, 5.3 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void k_mx4_quantize(const T* __restrict__ x, int64_t ldx, int64_t rows, int K, int nb,
                                                       uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
@@ -53,7 +54,8 @@ __global__ __launch_bounds__(256) void k_mx4_quantize(const T* __restrict__ x, i
     }
 }
 
-// A lane writes one 16-byte slot of the row (VEC codes).
+// A lane writes one 16-byte slot of the row (VEC codes): 12288 x 4096 bf16 20 us (6.4 TB/s); a block a lane, whose writes lie 64
+// bytes apart, took 31 us.
 template <typename T>
 __global__ __launch_bounds__(256) void k_mx4_dequantize(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows,
                                                         int K, int nb, T* __restrict__ y, int64_t ldy) {
@@ -92,6 +94,8 @@ __device__ const uint4 mx4_zero_block = {0u, 0u, 0u, 0u};
 // reads the fragments there.  A lane holds one block of a weight row and feeds it to four instructions, eight elements at a
 // time; the four lane groups hold different blocks, a permutation of the reduction index that x follows.  x comes from L2 for every
 // workgroup, which is why a wave takes NT weight tiles to one fragment of x.  The waves' sums meet in LDS in a fixed order.
+// Bound by the weight's bytes: 16 x 12288 x 4096 bf16 9.3 us (2.9 TB/s; an empty launch takes 3 us of it), 16 x 8192 x 8192 10.6 us
+// (3.4 TB/s).  fp32 rows have three parts, three times the instructions and the x traffic: 16 x 12288 x 4096 17 us.
 template <typename T, int MT, int NT, int NW>
 struct RowsStage {
     __attribute__((aligned(16))) uint8_t w[NW][NT * 1024], x[NW][MT * 16 * 128 * sizeof(T)];
@@ -225,7 +229,8 @@ __global__ __launch_bounds__(NW * 64) void k_mx4_rows(const T* __restrict__ x, i
     mx4_rows_store<T, MT, NT, NW>(reinterpret_cast<f32x4*>(&s0), acc, W, bias, btype, y, ldy, M, n0);
 }
 
-// The same product for rows of x that direct loads cannot take (not aligned to 16 bytes, or not whole chunks): fragments from memory.
+// The same product for rows of x that direct loads cannot take (not aligned to 16 bytes, or not whole chunks): fragments from memory,
+// a cache line a lane (16 x 4096 x 4096 bf16 16.5 us; aligned rows above 5.0 us).
 template <typename T, int MT, int NW>
 __global__ __launch_bounds__(NW * 64) void k_mx4_rows_any(const T* __restrict__ x, int64_t ldx, Mx4 W, const void* bias, int btype,
                                                           T* __restrict__ y, int64_t ldy, int M, int K) {
@@ -296,14 +301,18 @@ __device__ __forceinline__ void mx4_store_tile(float* strip, const f32x16 (&acc)
 }
 
 // ---- y = x W^T + bias and dx = dy W, many rows --------------------------------------------------------------------------
-// 128 x 128 outputs per workgroup, eight waves of 64 x 32 (32x32x16 bf16 matrix instructions), BK of the reduction per step, two
-// LDS stages.  Eight waves although four larger ones would read less from LDS: a single wave of a SIMD issues a vector
-// instruction every eight cycles only, two of them every four.  The float operand lies in LDS in its bf16 parts: rows of BK, 16-byte chunks in an order that spreads a fragment's rows over the banks; bf16 rows
-// whose chunks are aligned go there by direct loads, others through registers.
-//   y : the codes lie in LDS as they are and every wave widens the fragments it needs (an eighth of the LDS traffic of
-//       bf16 rows; the conversion instruction takes a quarter of the vector rate, half of the matrix instructions' time).
+// 128 x 128 outputs per workgroup, eight waves of 64 x 32 (32x32x16 bf16 matrix instructions), BK of the reduction per step, two or
+// three LDS stages.  Eight waves although four larger ones would read less from LDS: a single wave of a SIMD issues a vector
+// instruction every eight cycles only, two of them every four.  The float operand lies in LDS in its bf16 parts: rows of BK,
+// 16-byte chunks in an order that spreads a fragment's rows over the banks; bf16 rows whose chunks are aligned go there by direct
+// loads, others through registers.
+//   y : the codes lie in LDS as they are and every wave widens the fragments it needs (a quarter of the LDS traffic of bf16
+//       rows, for one conversion per two elements, at the rate of ordinary vector instructions, under the matrix instructions).
 //   dx: the reduction runs over W's rows, so that a fragment needs one column of eight rows: the block of a row is widened
 //       once, four rows side by side exchange their dwords (a transposition among four lanes), and the columns go to LDS.
+// bf16, y / dx: 1024 x 4096 x 4096 45 / 48 us (765 TFLOP/s; a library product of the same size with a bf16 weight 39 / 45 us),
+// 2048 x 8192 x 4096 153 / 168 us (900).  fp16 rows have two parts (82 / 88 us), fp32 rows three (120 / 120 us).  Bound by the
+// issue of vector and LDS instructions between the matrix instructions, which are busy 41% of the time.
 constexpr int TILE_WAVES = 8, TILE_THREADS = TILE_WAVES * 64;
 template <typename T, int BK, bool GRAD>
 struct TileStage {
@@ -619,6 +628,8 @@ __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__
 // An instruction's lane half h takes block 4 h + s of the step's eight in its s-th turn -- a permutation of the reduction index that
 // both operands share -- so that one dword holds a lane's four scales and the turn selects the byte.
 // Blocks behind the last one come from the zero block, rows behind the last one repeat it and are not stored.
+// 8192^3: 290 us, 3.8 PFLOP/s (matrix instructions busy 48% of the time, a third of the waves' time goes into waits for LDS and
+// loads); 4096^3: 45 to 47 us, 3.0; 1024 x 4096 x 4096: 19 us, 1.8 (a quarter of the tiles of the one before, on as many CUs).
 struct __attribute__((packed, aligned(1))) Bytes8 { uint32_t lo, hi; };
 
 template <int BM, int BN>
@@ -844,7 +855,8 @@ __global__ __launch_bounds__(256) void k_mx4_colsum(const T* __restrict__ dy, in
         if (c < N) part[(int64_t)blockIdx.y * N + c] = v;
     }
 }
-// about four workgroups a CU, of 32 rows at least
+// About four workgroups a CU, of 32 rows at least: 2048 x 8192 bf16 6.6 us (5.1 TB/s; 16 slices and one thread for each joined
+// column 17 us), 1024 x 4096 5.1 us (8 rows at least 6.8).
 static inline int mx4_colsum_slices(int M, int N) {
     const int64_t want = std::max<int64_t>(1, 1024 / ((N + 255ll) / 256));
     return (int)std::min<int64_t>(std::min<int64_t>(want, 256), (M + 31ll) / 32);
@@ -867,7 +879,8 @@ static int mx4_check_product(const char* what, const void* x, int64_t ldx, int d
     return DRM_OK;
 }
 // A reduction is split over workgroups where the tiles alone leave CUs idle: into about one workgroup a CU, of four steps at
-// least.  Returns the number of slices and the steps of each.
+// least.  64 x 4096 x 4096 bf16: 17 us, whole 30 us (gradient 18 and 40); where the launch of the join eats the gain the two are
+// even (1024 x 512 x 512 8 us both).  Returns the number of slices and the steps of each.
 static inline int mx4_split(int64_t tiles, int steps, int& span) {
     const int64_t want = tiles < 192 ? 256 / (tiles > 0 ? tiles : 1) : 1;
     const int slices = (int)std::max<int64_t>(1, std::min<int64_t>(want, steps / 4));
@@ -879,7 +892,8 @@ static inline size_t mx4_part_bytes(int slices, int M, int N) { return slices > 
 static inline int mx4_step_of(int dtype) { return dtype == DRM_BF16 ? 128 : 64; }
 
 // Large products: bf16 rows whose 16-byte chunks are aligned and whole go to LDS by direct loads with 128 of the reduction per step
-// (three stages where a row's scales are whole dwords); through registers the parts of wider types leave room for 64.
+// (1024 x 4096 x 4096 45.6 us, through registers 50.0; 2048 x 8192 x 4096 153 and 166), in three stages where a row's scales are
+// whole dwords (two: 46.2 and 156 us); through registers the parts of wider types leave room for 64.
 template <bool GRAD, typename T>
 static void mx4_launch_tile(const T* x, int64_t ldx, const Mx4& W, const void* bias, int btype, T* y, int64_t ldy, int M, int N, int K,
                             float* part, hipStream_t s) {
@@ -905,8 +919,11 @@ static void mx4_launch_tile(const T* x, int64_t ldx, const Mx4& W, const void* b
     if (!done) go(std::false_type{}, std::false_type{});
     if (part != nullptr) k_mx4_join<T><<<mx4_stream_grid((int64_t)M * ((N + 3) / 4)), 256, 0, s>>>(part, slices, M, N, bias, btype, y, ldy);
 }
-// Few rows: as many weight tiles per wave as leave about one workgroup a CU (x is read once per workgroup); eight waves where two
-// stages of their passes fit the LDS, else four.
+// Few rows: as many weight tiles per wave as leave about one workgroup a CU (x is read once per workgroup): bf16 16 x 12288 x 4096
+// with 1 / 2 / 4 tiles 11.4 / 11.5 / 9.3 us, 16 x 8192 x 8192 13.9 / 10.7 / 15.2 us, 16 x 4096 x 4096 5.1 / 6.1 / 8.8 us.  Eight
+// waves where two stages of their passes fit the LDS, else four (1 x 4096 x 4096 4.6 us, with four 5.1).  Up to 32 rows: 32 x 12288 x
+// 4096 12 us, the tiles above 21 us (16 rows 9.3 and 20 us, fp32 32 x 4096 x 4096 21.5 and 23.6 us); 33 rows would take three row
+// tiles and their tile kernel takes 15 us at 4096 x 4096.
 constexpr int MX4_FEW_ROWS = 32;
 template <typename T, int MT>
 static void mx4_launch_rows_mt(const T* x, int64_t ldx, const Mx4& W, const void* bias, int btype, T* y, int64_t ldy, int M, int N, int K, hipStream_t s) {
@@ -976,7 +993,9 @@ extern "C" int drm_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, i
     });
 }
 
-// the largest tile (fewest bytes through LDS per product) whose tiles still give most CUs one
+// The largest tile (fewest bytes through LDS per product) whose tiles still give most CUs one.  Tiles of 256 / 128 / 64: 4096^3 45 / 58 /
+// 85 us, 2048 x 6144 x 4096 (192 tiles of 256) 40 / 46 / 69 us, 1024 x 4096 x 4096 (256 of 128) 40 / 20 / 27 us, 257 x 1000 x 4080 20 / 12 /
+// 10 us.
 static int mx4_product_tile(int M, int N) { return mx4_tiles(M, N, 256) >= 192 ? 256 : mx4_tiles(M, N, 128) >= 192 ? 128 : 64; }
 
 static int mx4_check_workspace(const char* what, const void* ws, size_t have, size_t need) {

@@ -111,6 +111,17 @@ def test_absent_entries_and_empty_rows(V, rest):
 
 
 @pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [4097, 8195, 32771, 36867])
+def test_entries_at_the_ends_of_a_rows_pieces(V, dtype, rest):
+    s, values, idx, lse, g = inputs(3, V, 8, dtype, 1.0, rest)
+    idx[:] = torch.tensor([0, 4095, 4096, V - 1, V - 2, V - 3, V // 2, 31], device=DEV)
+    if rest:
+        lse = lse + 2.5
+    check(s, values, idx, 1.0, lse, g)
+
+
+@pytest.mark.parametrize("rest", [False, True])
 @pytest.mark.parametrize("V", [64, 3000, 40000])
 def test_an_index_listed_twice_adds_up(V, rest):
     s, values, idx, lse, g = inputs(4, V, 12, F32, 1.0, rest)
