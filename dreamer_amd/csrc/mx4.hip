@@ -312,7 +312,7 @@ __device__ __forceinline__ void mx4_store_tile(float* strip, const f32x16 (&acc)
 //       once, four rows side by side exchange their dwords (a transposition among four lanes), and the columns go to LDS.
 // bf16, y / dx: 1024 x 4096 x 4096 45 / 48 us (765 TFLOP/s; a library product of the same size with a bf16 weight 39 / 45 us),
 // 2048 x 8192 x 4096 153 / 168 us (900).  fp16 rows have two parts (82 / 88 us), fp32 rows three (120 / 120 us).  Bound by the
-// issue of vector and LDS instructions between the matrix instructions, which are busy 41% of the time.
+// issue of vector and LDS instructions between the matrix instructions, which are busy a third of the time.
 constexpr int TILE_WAVES = 8, TILE_THREADS = TILE_WAVES * 64;
 template <typename T, int BK, bool GRAD>
 struct TileStage {
@@ -628,7 +628,7 @@ __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__
 // An instruction's lane half h takes block 4 h + s of the step's eight in its s-th turn -- a permutation of the reduction index that
 // both operands share -- so that one dword holds a lane's four scales and the turn selects the byte.
 // Blocks behind the last one come from the zero block, rows behind the last one repeat it and are not stored.
-// 8192^3: 290 us, 3.8 PFLOP/s (matrix instructions busy 48% of the time, a third of the waves' time goes into waits for LDS and
+// 8192^3: 290 us, 3.8 PFLOP/s (matrix instructions busy 45 to 48% of the time, a third of the waves' time goes into waits for LDS and
 // loads); 4096^3: 45 to 47 us, 3.0; 1024 x 4096 x 4096: 19 us, 1.8 (a quarter of the tiles of the one before, on as many CUs).
 struct __attribute__((packed, aligned(1))) Bytes8 { uint32_t lo, hi; };
 

@@ -63,9 +63,16 @@ def quantize(x: torch.Tensor) -> MX4Tensor:
     return MX4Tensor._of(*N.mx4_quantize(rows), rows.shape[1])
 
 
+def _versions(w: MX4Tensor):
+    """Counts of in-place writes (tensors made under inference_mode have none)."""
+    return None if w.codes.is_inference() or w.scales.is_inference() else (w.codes._version, w.scales._version)
+
+
 def _mx4_linear_grads(ctx, dy):
     rows = N.as_rows(dy)
     w = ctx.weight
+    if ctx.versions != _versions(w):
+        raise N.NativeError("linear: the 4-bit weight was written to between the product and its gradient")
     dx = db = None
     if ctx.needs_input_grad[0]:
         dx = N.mx4_linear_dgrad(rows, w.codes, w.scales, w.columns)
@@ -82,6 +89,7 @@ class _MX4LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, bias, weight):
         ctx.weight = weight
+        ctx.versions = _versions(weight)
         ctx.bias_dtype = None if bias is None else bias.dtype
         y = N.mx4_linear(N.as_rows(x), weight.codes, weight.scales, bias)
         return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.codes.shape[0])

@@ -311,6 +311,19 @@ def test_layer_from_a_linear():
         both(x)
 
 
+def test_a_weight_written_to_before_its_gradient_is_refused():
+    w = weight(24, 64, 3)
+    x = torch.randn(3, 64, device=DEV, requires_grad=True)
+    y = mx4.linear(x, w)
+    w.scales.add_(1)
+    with pytest.raises(N.NativeError, match="written to"):
+        y.sum().backward()
+    with torch.inference_mode():
+        w = weight(24, 64, 3)
+    (dx,) = torch.autograd.grad(mx4.linear(x, w).sum(), x)
+    assert torch.equal(dx, torch.autograd.grad(mx4.linear(x, weight(24, 64, 3)).sum(), x)[0])
+
+
 def test_refusals_on_the_device():
     w = weight(24, 64, 9)
     x = torch.randn(3, 64, device=DEV)
