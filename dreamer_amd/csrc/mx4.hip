@@ -109,6 +109,12 @@ __device__ __forceinline__ void wait_loads() {        // no more than N vector m
     asm volatile("" ::: "memory");
 }
 
+// A barrier behind which every wave finds what the others brought to LDS: direct loads count as vector memory operations.
+__device__ __forceinline__ void stage_barrier() {
+    wait_loads<0>();
+    __syncthreads();
+}
+
 template <typename T, int MT, int NT, int NW>
 __device__ __forceinline__ void mx4_rows_store(f32x4* s_acc, const f32x4 (&acc)[NT][MT], const Mx4& W, const void* bias, int btype,
                                                T* __restrict__ y, int64_t ldy, int M, int n0) {
@@ -590,19 +596,19 @@ __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__
     } else if (steps > 0) {
         load(s0, begin, h, false);
         put(s0, begin, h, false);
-        __syncthreads();
+        stage_barrier();
         for (int p = 0; p < steps / 2; ++p) {
             const int k1 = begin + (2 * p + 1) * BK, k2 = k1 + BK;
             if constexpr (!GRAD) load_scales(k1, h);      // first: nothing behind it has to wait for the rest
             load(s1, k1, h, false);
             compute(s0);
             put(s1, k1, h, false);
-            __syncthreads();
+            stage_barrier();
             if constexpr (!GRAD) load_scales(k2, h);
             load(s0, k2, h, false);                       // behind the last step: not used
             compute(s1);
             put(s0, k2, h, false);
-            __syncthreads();
+            stage_barrier();
         }
         if (steps & 1) compute(s0);
     }
@@ -611,10 +617,10 @@ __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__
         if constexpr (!GRAD) { if (k0 > begin) load_scales(k0, h); }
         load(s1, k0, h, true);
         put(s1, k0, h, true);
-        __syncthreads();
+        stage_barrier();
         compute(s1);
     }
-    __syncthreads();
+    stage_barrier();
     float* strip = reinterpret_cast<float*>(&s0) + wave * 32 * OUT_LD;
     if (part != nullptr) mx4_store_tile<float, 64, WN>(strip, acc, part + (int64_t)blockIdx.y * M * N, N, m0 + wm, n0 + wn, M, N, nullptr, 0);
     else mx4_store_tile<T, 64, WN>(strip, acc, y, ldy, m0 + wm, n0 + wn, M, N, bias, btype);
@@ -771,22 +777,22 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void k_mx4_product(Mx4 
         const uint2 sx = mx4_short_row_scales(X, m0 + rx), sw = mx4_short_row_scales(W, n0 + rw);
         put(s0, second ? sw : sx, sw);
     }
-    __syncthreads();
+    stage_barrier();
     for (int p = 0; p < steps / 2; ++p) {
         const int kb1 = (first + 2 * p + 1) * 8, kb2 = kb1 + 8;
         scales(kb1, vx, vw);
         codes(s1, kb1);
         compute(s0);
         put_scales(s1, kb1, vx, vw);
-        __syncthreads();
+        stage_barrier();
         scales(kb2, vx, vw);
         codes(s0, kb2);                     // behind the last step: not used
         compute(s1);
         put_scales(s0, kb2, vx, vw);
-        __syncthreads();
+        stage_barrier();
     }
     if (steps & 1) compute(s0);
-    __syncthreads();
+    stage_barrier();
     float* strip = reinterpret_cast<float*>(&s0) + wave * 32 * OUT_LD;
     if (part != nullptr) {
         mx4_store_tile<float, WM, WN>(strip, acc, part + (int64_t)blockIdx.y * X.rows * W.rows, W.rows, m0 + wm, n0 + wn, X.rows, W.rows, nullptr, 0);
