@@ -804,6 +804,11 @@ def _workspace(device, name: str, *sizes: int):
     return (torch.empty(need // 4, dtype=torch.float32, device=device), need) if need else (None, 0)
 
 
+def wants_grad(a, b=None, c=None) -> bool:
+    """Whether a call with these tensors must leave a node in the autograd graph (one that need not is spared the node's cost)."""
+    return torch.is_grad_enabled() and (a.requires_grad or (b is not None and b.requires_grad) or (c is not None and c.requires_grad))
+
+
 def layer_norm_forward(x, weight, bias, eps: float, want_stats: bool):
     """LayerNorm over the rows of x (N, E); returns y (dense) and the rows' (mean, rstd) as (2, N) (None without ``want_stats``)."""
     xid = dtype_id(x, "x")

@@ -634,8 +634,10 @@ __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__
 // An instruction's lane half h takes block 4 h + s of the step's eight in its s-th turn -- a permutation of the reduction index that
 // both operands share -- so that one dword holds a lane's four scales and the turn selects the byte.
 // Blocks behind the last one come from the zero block, rows behind the last one repeat it and are not stored.
-// 8192^3: 290 us, 3.8 PFLOP/s (matrix instructions busy 45 to 48% of the time, a third of the waves' time goes into waits for LDS and
-// loads); 4096^3: 45 to 47 us, 3.0; 1024 x 4096 x 4096: 19 us, 1.8 (a quarter of the tiles of the one before, on as many CUs).
+// 8192^3: 290 to 304 us, 3.6 to 3.8 PFLOP/s; 4096^3: 45 to 48 us, 2.9; 1024 x 4096 x 4096: 20 us, 1.7 (tiles of 128).  The instructions alone,
+// from registers, reach 8.4 PFLOP/s with zeros but 5.7 to 6.5 with random codes, for which the clock falls (2.4 to below 2.0 GHz):
+// that, not the nominal rate, is the ceiling.  Matrix instructions are busy 45 to 48% of the time; without the loads from memory the
+// same loop takes 255 us, with a quarter of the LDS reads besides 214 us.
 struct __attribute__((packed, aligned(1))) Bytes8 { uint32_t lo, hi; };
 
 template <int BM, int BN>

@@ -187,7 +187,9 @@ def distill_topk_rows(logits: torch.Tensor, top_values: torch.Tensor, top_indice
     values, indices = _list_of(top_values, torch.float32, rows, k), _list_of(top_indices, torch.int64, rows, k)
     lse = None if top_lse is None else top_lse.detach().float().reshape(-1).contiguous()
     if logits.is_cuda:
-        return _DistillTopkRowsFn.apply(N.as_rows(logits), values, indices, lse, float(temperature))
+        if N.wants_grad(logits):
+            return _DistillTopkRowsFn.apply(N.as_rows(logits), values, indices, lse, float(temperature))
+        return N.distill_topk_forward(N.as_rows(logits), values, indices, lse, float(temperature))[0]
     N.dtype_id(logits, "logits")
     return _distill_topk_rows_host(logits.reshape(rows, -1).float(), values, indices, lse, float(temperature))
 

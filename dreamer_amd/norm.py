@@ -30,12 +30,9 @@ class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         rows = N.as_rows(x)
-        need = ctx.needs_input_grad
-        stats = need[0] or need[1] or need[2]
-        y, saved = N.layer_norm_forward(rows, weight, bias, eps, stats)
-        if stats:
-            ctx.save_for_backward(rows, weight, saved)
-            ctx.bias_dtype = None if bias is None else bias.dtype
+        y, stats = N.layer_norm_forward(rows, weight, bias, eps, True)
+        ctx.save_for_backward(rows, weight, stats)
+        ctx.bias_dtype = None if bias is None else bias.dtype
         return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
@@ -57,7 +54,10 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
             weight = weight.contiguous()
         if bias is not None and not bias.is_contiguous():
             bias = bias.contiguous()
-        return _LayerNormFn.apply(x, weight, bias, float(eps))
+        if N.wants_grad(x, weight, bias):
+            return _LayerNormFn.apply(x, weight, bias, float(eps))
+        y, _ = N.layer_norm_forward(N.as_rows(x), weight, bias, float(eps), False)
+        return y if x.dim() == 2 else y.view(x.shape)
     N.dtype_id(x, "x")
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and (t.shape != x.shape[-1:] or t.dtype not in (torch.float32, x.dtype) or t.device != x.device):
