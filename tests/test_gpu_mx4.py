@@ -245,6 +245,32 @@ def test_rows_beyond_32_bit_offsets():
     assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
 
 
+@pytest.mark.parametrize("M", [3, 40])
+def test_a_weight_beyond_32_bit_offsets(M):
+    rows, K, live = 1100003, 4096, 96
+    small = weight(live, K, 11)
+    codes = torch.zeros(rows, K // 2, dtype=torch.uint8, device=DEV)
+    scales = torch.full((rows, K // 32), 127, dtype=torch.uint8, device=DEV)
+    codes[-live:], scales[-live:] = small.codes, small.scales
+    w = mx4.MX4Tensor(codes, scales, K)
+    assert codes.numel() > 2 ** 31
+    x = torch.randn(M, K, device=DEV).to(BF16).requires_grad_()
+    y, ref = mx4.linear(x, w), mx4.linear(x, small)
+    # (a term is exact and the slices of a split reduction add up to the same sums in fp32 only up to rounding)
+    tol = 4096 * U * (x.detach().double().abs() @ small.dequantize().double().abs().T) + 2.0 ** -8 * ref.double().abs()
+    assert float(((y[:, -live:].double() - ref.double()).abs() - 2 * tol).max()) <= 0 and float(y[:, :-live].abs().max()) == 0
+    dy = torch.zeros(M, rows, dtype=BF16, device=DEV)
+    dy[:, -live:] = torch.randn(M, live, device=DEV)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    want = dy[:, -live:].double() @ small.dequantize().double()
+    tol = 4096 * U * (dy[:, -live:].double().abs() @ small.dequantize().double().abs()) + 2.0 ** -8 * want.abs()
+    assert float(((dx.double() - want).abs() - tol).max()) <= 0
+    q = mx4.quantize(x.detach())
+    assert torch.equal(mx4.linear(q, w)[:, -live:], mx4.linear(q, small)) or \
+        float((mx4.linear(q, w)[:, -live:].double() - mx4.linear(q, small).double()).abs().max()) <= 4096 * U * float((q.dequantize().double().abs() @ small.dequantize().double().abs().T).max())
+    assert torch.equal(w.dequantize(BF16)[-live:], small.dequantize(BF16))
+
+
 def test_empty_batches_and_absent_bias():
     w = weight(24, 64, 7)
     b = torch.ones(24, device=DEV, requires_grad=True)
