@@ -887,14 +887,20 @@ static int mx4_check_product(const char* what, const void* x, int64_t ldx, int d
     return DRM_OK;
 }
 // A reduction is split over workgroups where the tiles alone leave CUs idle: into about one workgroup a CU, of four steps at
-// least.  64 x 4096 x 4096 bf16: 17 us, whole 30 us (gradient 18 and 40); where the launch of the join eats the gain the two are
-// even (1024 x 512 x 512 8 us both).  Returns the number of slices and the steps of each.
-static inline int mx4_split(int64_t tiles, int steps, int& span) {
+// least, and only as far as the steps that this saves (step_us each) outweigh the join: its launch, 4 us with the host's side, and the
+// partial sums, written and read at 4 TB/s.  bf16 x: 64 x 4096 x 4096 17 us, whole 31 us (gradient 18 and 40), 64 x 4096 x 2048 13 and 17;
+// 512 x 2048 x 2048 would be 23 us in four slices, whole it is 18.  Both in 4 bits: 257 x 1000 x 8192 11 us, whole 15; x 4080 9.5 and 9.0.
+// Returns the number of slices and the steps of each.
+static inline int mx4_split(int64_t tiles, int steps, double step_us, int M, int N, int& span) {
     const int64_t want = tiles < 192 ? 256 / (tiles > 0 ? tiles : 1) : 1;
-    const int slices = (int)std::max<int64_t>(1, std::min<int64_t>(want, steps / 4));
+    int slices = (int)std::max<int64_t>(1, std::min<int64_t>(want, steps / 4));
+    while (slices > 1 && (steps - (steps + slices - 1) / slices) * step_us <= 4.0 + 2.0 * slices * M * N * sizeof(float) / 4e6) slices /= 2;
     span = (steps + slices - 1) / slices;
     return (steps + span - 1) / span;
 }
+// one step of a tile's workgroup, from products that were not split: 128 of the reduction for bf16 rows, 64 for the parts of the wider types
+static inline double mx4_step_us(int dtype) { return dtype == DRM_BF16 ? 0.85 : dtype == DRM_F16 ? 1.1 : 1.6; }
+constexpr double MX4_PRODUCT_STEP_US = 0.4;
 static inline int64_t mx4_tiles(int M, int N, int b) { return (int64_t)((M + b - 1) / b) * ((N + b - 1) / b); }
 static inline size_t mx4_part_bytes(int slices, int M, int N) { return slices > 1 ? (size_t)slices * M * N * sizeof(float) : 0; }
 static inline int mx4_step_of(int dtype) { return dtype == DRM_BF16 ? 128 : 64; }
@@ -908,7 +914,7 @@ static void mx4_launch_tile(const T* x, int64_t ldx, const Mx4& W, const void* b
     const int tm = (M + 127) / 128, tn = (N + 127) / 128;
     constexpr int BK = Parts<T>::N == 1 ? 128 : 64;
     int span = 0;
-    const int slices = mx4_split((int64_t)tm * tn, (K + BK - 1) / BK, span);
+    const int slices = mx4_split((int64_t)tm * tn, (K + BK - 1) / BK, mx4_step_us(Elem<T>::ID), M, N, span);
     if (slices == 1) part = nullptr;
     const dim3 grid(tm * tn, slices);
     auto go = [&](auto direct, auto ring) {
@@ -1016,18 +1022,18 @@ extern "C" size_t drm_mx4_linear_workspace_bytes(int32_t dtype, int32_t M, int32
     if (!elem_ok(dtype) || M <= MX4_FEW_ROWS || N < 1 || K < 1) return 0;
     int span = 0;
     const int bk = mx4_step_of(dtype);
-    return mx4_part_bytes(mx4_split(mx4_tiles(M, N, 128), (K - 1) / bk + 1, span), M, N);
+    return mx4_part_bytes(mx4_split(mx4_tiles(M, N, 128), (K - 1) / bk + 1, mx4_step_us(dtype), M, N, span), M, N);
 }
 extern "C" size_t drm_mx4_linear_dgrad_workspace_bytes(int32_t dtype, int32_t M, int32_t N, int32_t K) {
     if (!elem_ok(dtype) || M < 1 || N < 1 || K < 1) return 0;
     int span = 0;
     const int bk = mx4_step_of(dtype);
-    return mx4_part_bytes(mx4_split(mx4_tiles(M, K, 128), (N - 1) / bk + 1, span), M, K);
+    return mx4_part_bytes(mx4_split(mx4_tiles(M, K, 128), (N - 1) / bk + 1, mx4_step_us(dtype), M, K, span), M, K);
 }
 extern "C" size_t drm_mx4_product_workspace_bytes(int32_t M, int32_t N, int32_t K) {
     if (M < 1 || N < 1 || K < 1) return 0;
     int span = 0;
-    return mx4_part_bytes(mx4_split(mx4_tiles(M, N, mx4_product_tile(M, N)), (mx4_blocks(K) + 7) / 8, span), M, N);
+    return mx4_part_bytes(mx4_split(mx4_tiles(M, N, mx4_product_tile(M, N)), (mx4_blocks(K) + 7) / 8, MX4_PRODUCT_STEP_US, M, N, span), M, N);
 }
 
 extern "C" int drm_mx4_linear(const void* x, int64_t ldx, int32_t dtype, const uint8_t* codes, const uint8_t* scales, const void* bias,
@@ -1086,7 +1092,7 @@ extern "C" int drm_mx4_product(const uint8_t* x_codes, const uint8_t* x_scales, 
         using T = decltype(tag);
         const int b = mx4_product_tile(M, N), tm = (M + b - 1) / b, tn = (N + b - 1) / b;
         int span = 0;
-        const int slices = mx4_split((int64_t)tm * tn, (W.nb + 7) / 8, span);
+        const int slices = mx4_split((int64_t)tm * tn, (W.nb + 7) / 8, MX4_PRODUCT_STEP_US, M, N, span);
         float* part = slices > 1 ? (float*)workspace : nullptr;
         const dim3 grid(tm * tn, slices);
         if (b == 256) k_mx4_product<T, 256, 256, 128, 64><<<grid, 512, 0, s>>>(X, W, bias, bias_dtype, (T*)y, ldy, tm, tn, part, span);
