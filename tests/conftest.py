@@ -31,7 +31,8 @@ if GUARD:
     _guard.guard_report.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_ulonglong), ctypes.c_int]
 
 # tests that record torch.cuda graphs: the pluggable-allocator interface has no graph memory pools
-_NEEDS_GRAPH_POOLS = ("test_gpu_trainer.py", "test_flat_adam_in_a_recorded_graph")
+_NEEDS_GRAPH_POOLS = ("test_gpu_trainer.py", "test_flat_adam_in_a_recorded_graph", "test_on_another_stream_and_in_a_recorded_graph",
+                      "test_the_step_recorded_and_replayed")
 
 
 def guard_report(reset=True):
@@ -52,7 +53,8 @@ def pytest_configure(config):
 # DRM_SYNC_CHECK: the library synchronises after every launch, which a recording does not allow; the library and the
 # trainer then launch directly, and the tests that record library calls (or assert that a recording was made) have nothing to check
 _RECORDS_LIBRARY_CALLS = ("test_flat_adam_in_a_recorded_graph", "test_graph_replayed_updates_match_eager",
-                          "test_acting_policy_graph_replay_matches_eager_steps", "test_train_loop_end_to_end_on_the_gpu")
+                          "test_acting_policy_graph_replay_matches_eager_steps", "test_train_loop_end_to_end_on_the_gpu",
+                          "test_on_another_stream_and_in_a_recorded_graph", "test_the_step_recorded_and_replayed")
 SYNC_CHECK = os.environ.get("DRM_SYNC_CHECK", "0") not in ("", "0")
 
 
