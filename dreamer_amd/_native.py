@@ -11,6 +11,7 @@ import os
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DRM_LIB", os.path.join(_HERE, "libdreamer_amd.so"))
@@ -804,9 +805,18 @@ def _workspace(device, name: str, *sizes: int):
     return (torch.empty(need // 4, dtype=torch.float32, device=device), need) if need else (None, 0)
 
 
+def in_dual_level() -> bool:
+    """Whether forward-mode differentiation is under way (torch.autograd.forward_ad)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
 def wants_grad(a, b=None, c=None) -> bool:
-    """Whether a call with these tensors must leave a node in the autograd graph (one that need not is spared the node's cost)."""
-    return torch.is_grad_enabled() and (a.requires_grad or (b is not None and b.requires_grad) or (c is not None and c.requires_grad))
+    """Whether a call with these tensors must leave a node in the autograd graph (one that need not is spared the node's cost).  A
+    tensor with a forward-mode tangent counts (its ``requires_grad`` is False): the node refuses it, where the bare kernel would read
+    the values and drop the tangent."""
+    if torch.is_grad_enabled() and (a.requires_grad or (b is not None and b.requires_grad) or (c is not None and c.requires_grad)):
+        return True
+    return in_dual_level() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (a, b, c))
 
 
 def layer_norm_forward(x, weight, bias, eps: float, want_stats: bool):

@@ -130,8 +130,8 @@ class _DistillTopkRowsFn(torch.autograd.Function):
 
 
 def _list_of(t: torch.Tensor, dtype, rows: int, k: int) -> torch.Tensor:
-    """A list (rows, k), dense, in ``dtype``; the tensor itself where it is that."""
-    t = t.detach() if t.requires_grad else t
+    """A list (rows, k), dense, in ``dtype``, without derivatives; the tensor itself where it is that."""
+    t = t.detach() if t.requires_grad or N.in_dual_level() else t
     if t.dtype == dtype and t.dim() == 2 and t.is_contiguous():
         return t
     return t.to(dtype).reshape(rows, k).contiguous()

@@ -148,6 +148,6 @@ class MX4Linear(nn.Module):
         w = MX4Tensor(self.codes, self.scales, self.in_features)
         if self.activations == "float":
             return linear(x, w, self.bias)
-        if torch.is_grad_enabled() and (x.requires_grad or (self.bias is not None and self.bias.requires_grad)):
+        if N.wants_grad(x, self.bias):
             raise N.NativeError("MX4Linear: products of quantised rows have no gradient; call under torch.no_grad()")
         return linear(quantize(x), w, self.bias, x.dtype).view(*x.shape[:-1], self.out_features)

@@ -1,0 +1,33 @@
+"""What the layer norm, distillation and 4-bit operators promise beyond their values: derivatives are formed or refused, never lost."""
+import torch
+from torch.autograd import forward_ad
+
+from dreamer_amd import _native as N
+from dreamer_amd import losses
+
+
+def test_a_tensor_with_a_tangent_wants_its_derivative():
+    """A dual tensor has requires_grad == False; it must not pass for one without derivatives."""
+    x, w = torch.randn(4, 8), torch.ones(8)
+    assert not N.wants_grad(x) and not N.wants_grad(x, w, w)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        dual_w = forward_ad.make_dual(w, torch.ones_like(w))
+        assert not dual.requires_grad
+        for args in ((dual,), (x, dual_w), (x, w, dual_w), (x, None, dual_w)):
+            assert N.wants_grad(*args), args
+            with torch.no_grad():                       # switches off reverse mode only
+                assert N.wants_grad(*args), args
+        assert not N.wants_grad(x, w, None)
+
+
+def test_the_teacher_has_no_derivative_in_either_mode():
+    s, t = torch.randn(4, 8), torch.randn(4, 8)
+    values, idx = t.topk(3, 1)
+    lse = torch.logsumexp(t, 1)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(values, torch.ones_like(values))
+        assert forward_ad.unpack_dual(losses.distill_topk_rows(s, dual, idx)).tangent is None
+        assert forward_ad.unpack_dual(losses.distill_topk_rows(s, dual, idx, 1.0, forward_ad.make_dual(lse, lse))).tangent is None
+        moved = forward_ad.unpack_dual(losses.distill_topk_rows(forward_ad.make_dual(s, torch.ones_like(s)), values, idx)).tangent
+    assert moved is not None and float(moved.abs().max()) < 1e-5     # all logits moved alike: the softmax does not change
