@@ -18,18 +18,37 @@ from typing import Dict, Optional
 import torch
 
 from . import _native as N
+from .observe import check_sequence_model
 from .world_model import WorldModelState
 
 
-def _mlp_struct(mlp, head, in_dim: int) -> N.drm_mlp:
-    linears = [m for m in mlp if isinstance(m, torch.nn.Linear)]
-    norms = [m for m in mlp if isinstance(m, torch.nn.LayerNorm)]
+LN_EPS = 1e-5     # of every LayerNorm the rollout evaluates (the kernels hold it as a constant)
+
+
+def _mlp_struct(mlp, head, in_dim: int, name: str = "mlp") -> N.drm_mlp:
+    """Addresses of an MLP's parameters.  The kernels run (Linear, LayerNorm, SiLU) triples of one width and a Linear head; a model
+    with anything else in their place (a layer in 4 bits, a norm without weights) is refused, not read as if it were one."""
+    mods = list(mlp)
+    n = len(mods) // 3
+    if len(mods) != 3 * n or not 1 <= n <= N.DRM_MAX_MLP_LAYERS:
+        raise N.NativeError(f"{name}: {len(mods)} modules; the rollout runs 1 to {N.DRM_MAX_MLP_LAYERS} (Linear, LayerNorm, SiLU) triples")
     s = N.drm_mlp()
-    s.n_layers, s.in_dim, s.hidden, s.out_dim = len(linears), in_dim, linears[0].out_features, head.out_features
-    for i, (lin, ln) in enumerate(zip(linears, norms)):
-        s.w[i], s.b[i], s.ln_g[i], s.ln_b[i] = (lin.weight.data_ptr(), lin.bias.data_ptr(), ln.weight.data_ptr(),
-                                                ln.bias.data_ptr())
-    s.head_w, s.head_b = head.weight.data_ptr(), head.bias.data_ptr()
+    hidden = mods[0].out_features if isinstance(mods[0], torch.nn.Linear) else 0
+    for i in range(n):
+        lin, ln, act = mods[3 * i:3 * i + 3]
+        ok = (isinstance(lin, torch.nn.Linear) and isinstance(ln, torch.nn.LayerNorm) and isinstance(act, torch.nn.SiLU)
+              and lin.in_features == (hidden if i else in_dim) and lin.out_features == hidden and tuple(ln.normalized_shape) == (hidden,)
+              and ln.eps == LN_EPS)
+        tensors = [m._parameters.get(k) for m in (lin, ln) for k in ("weight", "bias")] if ok else [None]
+        if any(t is None for t in tensors):
+            raise N.NativeError(f"{name}: the rollout runs Linear({hidden if i else in_dim}, width), LayerNorm(width, eps={LN_EPS}) and SiLU, "
+                                f"each with its parameters, not {lin}, {ln}, {act}")
+        s.w[i], s.b[i], s.ln_g[i], s.ln_b[i] = (t.data_ptr() for t in tensors)
+    tensors = [head._parameters.get(k) for k in ("weight", "bias")] if isinstance(head, torch.nn.Linear) and head.in_features == hidden else [None]
+    if any(t is None for t in tensors):
+        raise N.NativeError(f"{name}: the rollout runs a Linear head of {hidden} inputs with a bias, not {head}")
+    s.n_layers, s.in_dim, s.hidden, s.out_dim = n, in_dim, hidden, head.out_features
+    s.head_w, s.head_b = (t.data_ptr() for t in tensors)
     return s
 
 
@@ -82,15 +101,16 @@ class ImagineEngine:
         S = d.D + d.L * d.K
         w = N.drm_imagine_weights()
         w.dims = d
+        check_sequence_model(wm)
         w.a_emb, w.lin_w, w.lin_b = wm.seq.a_emb.weight.data_ptr(), wm.seq.linear.weight.data_ptr(), wm.seq.linear.bias.data_ptr()
         g = wm.seq.gru
         w.gru_w_ih, w.gru_w_hh, w.gru_b_ih, w.gru_b_hh = (g.weight_ih.data_ptr(), g.weight_hh.data_ptr(),
                                                          g.bias_ih.data_ptr(), g.bias_hh.data_ptr())
-        w.dyn = _mlp_struct(wm.dyn.mlp, wm.dyn.head, d.D)
-        w.rew = _mlp_struct(wm.rew.mlp, wm.rew.head, S)
-        w.cont = _mlp_struct(wm.cont.mlp, wm.cont.head, S)
-        w.actor = _mlp_struct(self.actor.mlp, self.actor.head, S)
-        w.critic = _mlp_struct(self.critic.mlp, self.critic.head, S)
+        w.dyn = _mlp_struct(wm.dyn.mlp, wm.dyn.head, d.D, "dyn")
+        w.rew = _mlp_struct(wm.rew.mlp, wm.rew.head, S, "rew")
+        w.cont = _mlp_struct(wm.cont.mlp, wm.cont.head, S, "cont")
+        w.actor = _mlp_struct(self.actor.mlp, self.actor.head, S, "actor")
+        w.critic = _mlp_struct(self.critic.mlp, self.critic.head, S, "critic")
         w.buckets = self.critic.buckets.data_ptr()
         w.pack, w.pack_bytes = self.pack.data_ptr(), self.pack.numel() * 4
         return w

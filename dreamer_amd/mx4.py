@@ -129,7 +129,9 @@ def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[
 
 class MX4Linear(nn.Module):
     """A Linear layer whose frozen weight is held in 4 bits (``from_linear`` quantises one).  ``activations="mx4"`` also quantises
-    the rows, without gradients; ``"float"`` (default) multiplies them as they are."""
+    the rows, without gradients; ``"float"`` (default) multiplies them as they are.  A layer of this kind works in models that are
+    evaluated module by module; the rollout and the recurrence kernels (``imagine``, ``observe``) read float weights and refuse a
+    model in which it stands for one of their Linears."""
 
     def __init__(self, weight: MX4Tensor, bias: Optional[torch.Tensor] = None, activations: str = "float"):
         super().__init__()

@@ -65,6 +65,22 @@ def _wgrad_bf16(dy, x):
     return N.fused_linear(dy.t().contiguous(), x.t().contiguous(), bf16=True)
 
 
+def check_sequence_model(wm) -> None:
+    """The kernels read the recurrence's parameters by address: a model with another kind of layer in place of one (a Linear in
+    4 bits, other widths) is refused."""
+    from . import _native as N
+    seq, D, LK = wm.seq, wm.hidden_size, wm.num_latents * wm.classes_per_latent
+    emb, lin, gru = seq.a_emb, seq.linear, seq.gru
+    if not (isinstance(emb, torch.nn.Embedding) and emb.num_embeddings == wm.action_size and emb._parameters.get("weight") is not None):
+        raise N.NativeError(f"seq.a_emb: the recurrence reads an Embedding of {wm.action_size} actions, not {emb}")
+    if not (isinstance(lin, torch.nn.Linear) and lin.in_features == LK + emb.embedding_dim and lin.out_features == D
+            and lin._parameters.get("weight") is not None and lin._parameters.get("bias") is not None):
+        raise N.NativeError(f"seq.linear: the recurrence reads a Linear({LK + emb.embedding_dim}, {D}) with a bias, not {lin}")
+    if not (isinstance(gru, torch.nn.GRUCell) and gru.input_size == D and gru.hidden_size == D
+            and all(gru._parameters.get(k) is not None for k in ("weight_ih", "weight_hh", "bias_ih", "bias_hh"))):
+        raise N.NativeError(f"seq.gru: the recurrence reads a GRUCell({D}, {D}) with biases, not {gru}")
+
+
 class _ObserveEngine:
     """Packed tables and workspace of one world model for the native scan."""
 
@@ -207,6 +223,7 @@ def observe_scan(wm, e_part, a_prev, c_prev, expo_reset, expo_z, state, engine_a
         return _scan_eager(wm, e_part, a_prev, c_prev, expo_reset, expo_z, state)
     from . import _native as N
     from .world_model import WorldModelState
+    check_sequence_model(wm)
     eng = getattr(wm, engine_attr, None)
     if eng is None:
         eng = _ObserveEngine(wm)
@@ -217,8 +234,10 @@ def observe_scan(wm, e_part, a_prev, c_prev, expo_reset, expo_z, state, engine_a
     eng.precision = 1 if (prec == "bf16" and wm.hidden_size > 512) else 0
     B, T = a_prev.shape
     L, K = wm.num_latents, wm.classes_per_latent
-    g = wm.seq.gru
-    fc_w_h = wm.enc.fc[0].weight[:, wm.enc.conv_out_size:]
+    g, fc = wm.seq.gru, wm.enc.fc[0]
+    if not (isinstance(fc, torch.nn.Linear) and fc.in_features == wm.enc.conv_out_size + wm.hidden_size and fc.out_features == L * K):
+        raise N.NativeError(f"enc.fc[0]: the recurrence reads a Linear({wm.enc.conv_out_size + wm.hidden_size}, {L * K}), not {fc}")
+    fc_w_h = fc.weight[:, wm.enc.conv_out_size:]
     zidx0 = N.onehot_to_index(state.z.detach().contiguous().float())
     h, z, post, zidx = ObserveScanFn.apply(eng, e_part, wm.seq.a_emb.weight, wm.seq.linear.weight, wm.seq.linear.bias,
                                            g.weight_ih, g.weight_hh, g.bias_ih, g.bias_hh, fc_w_h, state.h.detach(), zidx0,
