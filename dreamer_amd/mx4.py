@@ -63,20 +63,19 @@ def quantize(x: torch.Tensor) -> MX4Tensor:
     return MX4Tensor._of(*N.mx4_quantize(rows), rows.shape[1])
 
 
-def _versions(w: MX4Tensor):
+def _versions(codes: torch.Tensor, scales: torch.Tensor):
     """Counts of in-place writes (tensors made under inference_mode have none)."""
-    return None if w.codes.is_inference() or w.scales.is_inference() else (w.codes._version, w.scales._version)
+    return None if codes.is_inference() or scales.is_inference() else (codes._version, scales._version)
 
 
 def _mx4_linear_grads(ctx, dy):
     rows = N.as_rows(dy)
-    w = ctx.weight
-    if ctx.versions != _versions(w):
+    if ctx.versions != _versions(ctx.codes, ctx.scales):
         raise N.NativeError("linear: the 4-bit weight was written to between the product and its gradient")
     dx = db = None
     if ctx.needs_input_grad[0]:
-        dx = N.mx4_linear_dgrad(rows, w.codes, w.scales, w.columns)
-        dx = dx if dy.dim() == 2 else dx.view(*dy.shape[:-1], w.columns)
+        dx = N.mx4_linear_dgrad(rows, ctx.codes, ctx.scales, ctx.columns)
+        dx = dx if dy.dim() == 2 else dx.view(*dy.shape[:-1], ctx.columns)
     if ctx.needs_input_grad[1]:
         db = N.mx4_bias_grad(rows, ctx.bias_dtype)
     return dx, db, None
@@ -88,8 +87,10 @@ _mx4_linear_grads_once = once_differentiable(_mx4_linear_grads)
 class _MX4LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, bias, weight):
-        ctx.weight = weight
-        ctx.versions = _versions(weight)
+        # the tensors of this product: the caller may put others into the MX4Tensor afterwards (kept as attributes, since tensors
+        # made under inference_mode cannot be saved for backward)
+        ctx.codes, ctx.scales, ctx.columns = weight.codes, weight.scales, weight.columns
+        ctx.versions = _versions(ctx.codes, ctx.scales)
         ctx.bias_dtype = None if bias is None else bias.dtype
         y = N.mx4_linear(N.as_rows(x), weight.codes, weight.scales, bias)
         return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.codes.shape[0])

@@ -36,3 +36,17 @@ def test_forward_mode_derivatives_are_refused():
         loss = losses.distill_topk_rows(x, dual(values), idx)
         assert forward_ad.unpack_dual(loss).tangent is None and torch.equal(loss, losses.distill_topk_rows(x, values, idx))
         assert torch.equal(norm.layer_norm(x, w, b), plain)
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+def test_a_4_bit_weight_that_is_exchanged_keeps_the_gradient_of_the_product(rows):
+    """Other tensors put into the MX4Tensor between the product and its gradient (a weight that is quantised anew)."""
+    for columns in (64, 96):
+        w, other = mx4.quantize(torch.randn(24, 64, device=DEV)), mx4.quantize(torch.randn(24, columns, device=DEV))
+        x = torch.randn(rows, 64, device=DEV, requires_grad=True)
+        dy = torch.randn(rows, 24, device=DEV)
+        (want,) = torch.autograd.grad(mx4.linear(x, w), x, dy)
+        y = mx4.linear(x, w)
+        w.codes, w.scales, w.columns = other.codes, other.scales, columns
+        (dx,) = torch.autograd.grad(y, x, dy)
+        assert torch.equal(dx, want)
