@@ -101,21 +101,44 @@ class _MX4LinearFn(torch.autograd.Function):
         return _mx4_linear_grads_once(ctx, dy) if torch.is_grad_enabled() else _mx4_linear_grads(ctx, dy)
 
 
+def _mx4_product_grad(ctx, dy):
+    return N.mx4_bias_grad(N.as_rows(dy), ctx.bias_dtype), None, None, None
+
+
+_mx4_product_grad_once = once_differentiable(_mx4_product_grad)
+
+
+class _MX4ProductFn(torch.autograd.Function):
+    """The product of rows and weight that are both in 4 bits, for the gradient of its bias."""
+
+    @staticmethod
+    def forward(ctx, bias, x, weight, out_dtype):
+        ctx.bias_dtype = bias.dtype
+        return N.mx4_product(x.codes, x.scales, weight.codes, weight.scales, weight.columns, bias, out_dtype)
+
+    @staticmethod
+    def backward(ctx, dy):
+        return _mx4_product_grad_once(ctx, dy) if torch.is_grad_enabled() else _mx4_product_grad(ctx, dy)
+
+
 def linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[torch.Tensor] = None,
            out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x @ weight.T + bias for a weight (N, K) in 4 bits.
 
     x a float tensor (..., K), fp32 / bf16 / fp16: the result has x's type (``out_dtype`` may only repeat it); each product is exact,
     sums are fp32.  Differentiable with respect to x and bias (once); the weight is frozen.
-    x an MX4Tensor (M, K): the result is (M, N) in ``out_dtype`` (default fp32); not differentiable.
+    x an MX4Tensor (M, K): the result is (M, N) in ``out_dtype`` (default fp32); differentiable with respect to bias only (once).
     bias (N,) in any of the three types."""
     if not isinstance(weight, MX4Tensor):
         raise N.NativeError(f"linear: the weight must be an MX4Tensor, got {type(weight).__name__}")
     if isinstance(x, MX4Tensor):
         if x.columns != weight.columns:
             raise N.NativeError(f"linear: rows of {x.columns} elements, weight {tuple(weight.shape)}")
-        return N.mx4_product(x.codes, x.scales, weight.codes, weight.scales, weight.columns, None if bias is None else bias.detach().contiguous(),
-                             out_dtype or torch.float32)
+        if bias is not None:
+            bias = bias if bias.is_contiguous() else bias.contiguous()
+            if N.wants_grad(bias):
+                return _MX4ProductFn.apply(bias, x, weight, out_dtype or torch.float32)
+        return N.mx4_product(x.codes, x.scales, weight.codes, weight.scales, weight.columns, bias, out_dtype or torch.float32)
     if x.dim() < 1 or x.shape[-1] != weight.columns:
         raise N.NativeError(f"linear: rows {tuple(x.shape)}, weight {tuple(weight.shape)}")
     if out_dtype is not None and out_dtype != x.dtype:

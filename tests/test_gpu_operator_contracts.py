@@ -50,3 +50,25 @@ def test_a_4_bit_weight_that_is_exchanged_keeps_the_gradient_of_the_product(rows
         w.codes, w.scales, w.columns = other.codes, other.scales, columns
         (dx,) = torch.autograd.grad(y, x, dy)
         assert torch.equal(dx, want)
+
+
+@pytest.mark.parametrize("dtype,bias_dtype", [(F32, F32), (BF16, F32), (BF16, BF16), (F16, F16)])
+@pytest.mark.parametrize("rows", [1, 5, 300])
+def test_a_product_of_4_bit_rows_has_its_bias_gradient(rows, dtype, bias_dtype):
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    a, w = mx4.quantize(torch.randn(rows, 96, generator=g, device=DEV)), mx4.quantize(torch.randn(40, 96, generator=g, device=DEV))
+    b = torch.randn(2, 40, generator=g, device=DEV).to(bias_dtype).t()[:, 0].requires_grad_()       # (not contiguous)
+    y = mx4.linear(a, w, b, out_dtype=dtype)
+    dy = torch.randn(rows, 40, generator=g, device=DEV).to(dtype)
+    (db,) = torch.autograd.grad(y, b, dy, retain_graph=True)
+    ref = dy.double().sum(0)
+    tol = torch.finfo(bias_dtype).eps / 2 * ref.abs() + rows * U * dy.double().abs().sum(0)          # rows additions in fp32, one rounding
+    assert db.dtype == bias_dtype and float(((db.double() - ref).abs() - tol).max()) <= 0
+    (gb,) = torch.autograd.grad(y, b, dy, create_graph=True)
+    with pytest.raises(RuntimeError):
+        gb.sum().backward()
+    with torch.no_grad():
+        plain = mx4.linear(a, w, b, out_dtype=dtype)
+    assert torch.equal(plain, y.detach()) and not plain.requires_grad and not mx4.linear(a, w).requires_grad
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+        mx4.linear(a, w, forward_ad.make_dual(b.detach(), torch.ones(40, device=DEV, dtype=bias_dtype)))
