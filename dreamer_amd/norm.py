@@ -45,7 +45,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x (any leading shape; rows may be strided).
 
-    x in fp32, bf16 or fp16; weight and bias (E,) in fp32 or in x's type, or None.  The result is dense, in x's type, and
+    x in fp32, bf16 or fp16; weight and bias (E,), or None, both in fp32 or both in x's type.  The result is dense, in x's type, and
     differentiable with respect to x, weight and bias (once)."""
     if x.dim() < 1 or x.shape[-1] < 1:
         raise N.NativeError(f"layer_norm: rows of at least one element, got shape {tuple(x.shape)}")
@@ -62,6 +62,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and (t.shape != x.shape[-1:] or t.dtype not in (torch.float32, x.dtype) or t.device != x.device):
             raise N.NativeError(f"layer_norm: {name} {tuple(t.shape)} {t.dtype} on {t.device} does not fit rows {tuple(x.shape)} {x.dtype}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise N.NativeError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
     v = x.float()
     c = v - v.mean(-1, keepdim=True)
     y = c * torch.rsqrt(c.square().mean(-1, keepdim=True) + eps)

@@ -1,9 +1,10 @@
 """What the layer norm, distillation and 4-bit operators promise beyond their values: derivatives are formed or refused, never lost."""
+import pytest
 import torch
 from torch.autograd import forward_ad
 
 from dreamer_amd import _native as N
-from dreamer_amd import losses
+from dreamer_amd import losses, norm
 
 
 def test_a_tensor_with_a_tangent_wants_its_derivative():
@@ -31,3 +32,13 @@ def test_the_teacher_has_no_derivative_in_either_mode():
         assert forward_ad.unpack_dual(losses.distill_topk_rows(s, dual, idx, 1.0, forward_ad.make_dual(lse, lse))).tangent is None
         moved = forward_ad.unpack_dual(losses.distill_topk_rows(forward_ad.make_dual(s, torch.ones_like(s)), values, idx)).tangent
     assert moved is not None and float(moved.abs().max()) < 1e-5     # all logits moved alike: the softmax does not change
+
+
+def test_layer_norm_takes_weight_and_bias_of_one_type():
+    """As on the device (a tensor that moves there must not be refused by a call that worked before)."""
+    x, one = torch.randn(4, 8).bfloat16(), torch.ones(8)
+    for w, b in ((one, one.bfloat16()), (one.bfloat16(), one)):
+        with pytest.raises(N.NativeError, match="weight is"):
+            norm.layer_norm(x, w, b)
+    for w, b in ((one, one), (one.bfloat16(), one.bfloat16()), (one, None), (None, one.bfloat16())):
+        assert norm.layer_norm(x, w, b).dtype == torch.bfloat16
