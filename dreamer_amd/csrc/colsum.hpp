@@ -5,12 +5,13 @@
 namespace drm {
 
 // 32 columns x 32 groups of slices per workgroup (short of bytes and long of latency: eight loads under way per thread; 1024 x 8192
-// sums 10 us, against 90 with a thread per column), groups added in order.  Column c < first: a[c], else b[c - first].
+// sums 10 us, against 90 with a thread per column), groups added in order.  Workgroups beyond 2^21 along the second axis (a launch takes
+// fewer than 2^32 threads along one).  Column c < first: a[c], else b[c - first].
 static __global__ __launch_bounds__(1024) void k_join_columns(const float* __restrict__ partials, int slices, int64_t cols, int64_t first, int type,
                                                               void* a, void* b) {
     __shared__ float s_part[32][33];
     const int g = threadIdx.x >> 5, l = threadIdx.x & 31;
-    const int64_t c = (int64_t)blockIdx.x * 32 + l;
+    const int64_t c = (((int64_t)blockIdx.y << 21) + blockIdx.x) * 32 + l;
     float sum[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) sum[u] = 0.f;
@@ -36,7 +37,8 @@ static __global__ __launch_bounds__(1024) void k_join_columns(const float* __res
     }
 }
 static inline void join_columns(const float* partials, int slices, int64_t cols, int64_t first, int type, void* a, void* b, hipStream_t s) {
-    k_join_columns<<<(unsigned)((cols + 31) / 32), 1024, 0, s>>>(partials, slices, cols, first, type, a, b);
+    const int64_t groups = (cols + 31) / 32, row = (int64_t)1 << 21;
+    k_join_columns<<<dim3((unsigned)(groups < row ? groups : row), (unsigned)((groups + row - 1) / row)), 1024, 0, s>>>(partials, slices, cols, first, type, a, b);
 }
 
 }  // namespace drm

@@ -22,6 +22,7 @@
 // up to three exponentials in 64 bits by one wave, about 1.5 us of a SIMD (65536 x 1024: 96 us, with the rest 152 us, 1.4 and 0.9 TB/s).
 #include "elem.hpp"
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -44,6 +45,13 @@ struct DistillArgs {
     int segs;
     float4* part;                      // (rows, segs): maximum m and sum of exp((s - m) / T) of the unlisted, of the listed entries
     float* loss; float* p; DistillRow* row;
+    template <typename T> DistillArgs from(int64_t r) const {      // the rows from r on
+        DistillArgs a = *this;
+        a.s = (const T*)s + r * lds; a.val += r * ldv; a.idx += r * ldi; a.loss += r; a.p += r * k; a.row += r;
+        if (lse != nullptr) a.lse += r;
+        if (part != nullptr) a.part += r * segs;
+        return a;
+    }
 };
 
 // exp(d / T) for d <= 0 as 2^(d c), c = log2(e) / T rounded to 32 bits.  The per-row scalars take c ln(2) in 64 bits as the
@@ -274,6 +282,11 @@ struct DistillBwdArgs {
     const int64_t* idx; int64_t ldi; int k;
     const float* p; const DistillRow* row; const float* g;
     void* ds; float inv_t; int segs;
+    template <typename T> DistillBwdArgs from(int64_t r) const {
+        DistillBwdArgs a = *this;
+        a.s = (const T*)s + r * lds; a.idx += r * ldi; a.p += r * k; a.row += r; a.g += r; a.ds = (T*)ds + r * V;
+        return a;
+    }
 };
 
 // One workgroup per (row, segment): the stream first, then the listed entries over what it wrote (same workgroup, behind a
@@ -376,12 +389,16 @@ extern "C" int drm_distill_topk_forward(const void* logits, int64_t ld_logits, i
     ProfScope ps(PC_ELEMENTWISE, s, 6 * n, n * elem_bytes(dtype) + (double)rows * k * 12);
     return with_elem(dtype, [&](auto tag) -> int {
         using T = decltype(tag);
-        const int grid = (int)(rows * A.segs);
         // one wave a row: more rows under way (8192 x 4096 bf16 21 us, four waves a row 34); few longer rows want the four (256 x
         // 8192: 7.5 and 6.0 us)
-        if (V <= 4096) k_distill_fwd<T, 64><<<grid, 64, 0, s>>>(A, c);
-        else k_distill_fwd<T, 256><<<grid, 256, 0, s>>>(A, c);
-        DRM_LAUNCH_CHECK();
+        const int64_t most = launch_limit(V <= 4096 ? 64 : 256) / A.segs;
+        for (int64_t r = 0; r < rows; r += most) {
+            const DistillArgs P = A.from<T>(r);
+            const int grid = (int)(std::min(rows - r, most) * A.segs);
+            if (V <= 4096) k_distill_fwd<T, 64><<<grid, 64, 0, s>>>(P, c);
+            else k_distill_fwd<T, 256><<<grid, 256, 0, s>>>(P, c);
+            DRM_LAUNCH_CHECK();
+        }
         if (A.segs > 1) {
             k_distill_join<T><<<(int)rows, 64, 0, s>>>(A);
             DRM_LAUNCH_CHECK();
@@ -405,11 +422,15 @@ extern "C" int drm_distill_topk_backward(const void* logits, int64_t ld_logits, 
     ProfScope ps(PC_ELEMENTWISE, s, 5 * n, 2 * n * elem_bytes(dtype) + (double)rows * k * 12);
     return with_elem(dtype, [&](auto tag) -> int {
         using T = decltype(tag);
-        const int grid = (int)(rows * A.segs);
         // (32768 x 1024 bf16: one wave 35 us, four 46; 1024 x 4096: 6.5 and 5.3)
-        if (V <= 2048) k_distill_bwd<T, 64><<<grid, 64, 0, s>>>(A, c);
-        else k_distill_bwd<T, 256><<<grid, 256, 0, s>>>(A, c);
-        DRM_LAUNCH_CHECK();
+        const int64_t most = launch_limit(V <= 2048 ? 64 : 256) / A.segs;
+        for (int64_t r = 0; r < rows; r += most) {
+            const DistillBwdArgs P = A.from<T>(r);
+            const int grid = (int)(std::min(rows - r, most) * A.segs);
+            if (V <= 2048) k_distill_bwd<T, 64><<<grid, 64, 0, s>>>(P, c);
+            else k_distill_bwd<T, 256><<<grid, 256, 0, s>>>(P, c);
+            DRM_LAUNCH_CHECK();
+        }
         return DRM_OK;
     });
 }

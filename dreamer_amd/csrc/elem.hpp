@@ -16,6 +16,10 @@ template <> struct Elem<_Float16> { static constexpr int VEC = 8; static constex
 static inline size_t elem_bytes(int dtype) { return dtype == DRM_F32 ? 4 : 2; }
 static inline bool elem_ok(int dtype) { return dtype == DRM_F32 || dtype == DRM_BF16 || dtype == DRM_F16; }
 
+// A launch takes fewer than 2^32 threads along an axis: the most workgroups of `threads` that one can have.  Kernels with a workgroup
+// per row or tile are launched more than once beyond that (a second grid axis in the kernels costs them 3 to 5%).
+static inline int64_t launch_limit(int threads) { return ((int64_t)1 << 32) / threads - 1; }
+
 // one 16-byte slot of VEC elements, aligned like a single element (global memory takes dword accesses at any byte address)
 template <typename T>
 struct __attribute__((packed, aligned(sizeof(T)))) Slot { T v[Elem<T>::VEC]; };

@@ -958,14 +958,22 @@ static void mx4_launch_rows_mt(const T* x, int64_t ldx, const Mx4& W, const void
 }
 template <typename T>
 static void mx4_launch_rows(const T* x, int64_t ldx, const Mx4& W, const void* bias, int btype, T* y, int64_t ldy, int M, int N, int K, hipStream_t s) {
-    if (M <= 16) mx4_launch_rows_mt<T, 1>(x, ldx, W, bias, btype, y, ldy, M, N, K, s);
-    else mx4_launch_rows_mt<T, 2>(x, ldx, W, bias, btype, y, ldy, M, N, K, s);
+    // (as many rows of the weight as one launch of 16 rows for 512 threads takes)
+    const int64_t most = launch_limit(512) * 16;
+    for (int64_t n = 0; n < N; n += most) {
+        const int rows = (int)std::min<int64_t>(N - n, most);
+        const Mx4 P{W.codes + n * W.nb * 16, W.scales + n * W.nb, rows, W.nb};
+        const void* b = bias != nullptr ? (const char*)bias + n * elem_bytes(btype) : nullptr;
+        if (M <= 16) mx4_launch_rows_mt<T, 1>(x, ldx, P, b, btype, y + n, ldy, M, rows, K, s);
+        else mx4_launch_rows_mt<T, 2>(x, ldx, P, b, btype, y + n, ldy, M, rows, K, s);
+    }
 }
 
-static int mx4_check_tiles(const char* what, int M, int N, int K) {
+static int mx4_check_tiles(const char* what, int M, int N, int K, int tile) {
     DRM_REQUIRE(K <= (1 << 22), DRM_ENOTSUP, "%s: a row of %d elements (at most 4194304)", what, K);
     DRM_REQUIRE(M <= 65535 * 128, DRM_ENOTSUP, "%s: M=%d rows (at most %d)", what, M, 65535 * 128);
-    DRM_REQUIRE(((int64_t)M + 127) / 128 * (((int64_t)N + 127) / 128) <= INT_MAX / 4, DRM_ENOTSUP, "%s: M=%d N=%d: too many tiles", what, M, N);
+    // (of 512 threads, and a launch takes fewer than 2^32 along an axis; 0: no tiles)
+    DRM_REQUIRE(tile == 0 || mx4_tiles(M, N, tile) < 1 << 23, DRM_ENOTSUP, "%s: M=%d N=%d: too many tiles", what, M, N);
     return DRM_OK;
 }
 
@@ -1042,7 +1050,7 @@ extern "C" int drm_mx4_linear(const void* x, int64_t ldx, int32_t dtype, const u
     if (M == 0 && N >= 1 && K >= 1) return DRM_OK;
     if (int rc = mx4_check(__func__, codes, scales, N, K)) return rc;
     if (int rc = mx4_check_product(__func__, x, ldx, dtype, K, bias, bias_dtype, y, ldy, N, M)) return rc;
-    if (int rc = mx4_check_tiles(__func__, M, N, K)) return rc;
+    if (int rc = mx4_check_tiles(__func__, M, N, K, M <= MX4_FEW_ROWS ? 0 : 128)) return rc;
     if (int rc = mx4_check_workspace(__func__, workspace, workspace_bytes, drm_mx4_linear_workspace_bytes(dtype, M, N, K))) return rc;
     hipStream_t s = (hipStream_t)stream;
     const Mx4 W{codes, scales, N, mx4_blocks(K)};
@@ -1062,7 +1070,7 @@ extern "C" int drm_mx4_linear_dgrad(const void* dy, int64_t lddy, int32_t dtype,
     if (M == 0 && N >= 1 && K >= 1) return DRM_OK;
     if (int rc = mx4_check(__func__, codes, scales, N, K)) return rc;
     if (int rc = mx4_check_product(__func__, dy, lddy, dtype, N, nullptr, 0, dx, lddx, K, M)) return rc;
-    if (int rc = mx4_check_tiles(__func__, M, K, K)) return rc;
+    if (int rc = mx4_check_tiles(__func__, M, K, K, 128)) return rc;
     DRM_REQUIRE(N >= 1 && N <= (1 << 30), DRM_EINVAL, "N=%d", N);
     if (int rc = mx4_check_workspace(__func__, workspace, workspace_bytes, drm_mx4_linear_dgrad_workspace_bytes(dtype, M, N, K))) return rc;
     hipStream_t s = (hipStream_t)stream;
@@ -1083,7 +1091,7 @@ extern "C" int drm_mx4_product(const uint8_t* x_codes, const uint8_t* x_scales, 
     if (int rc = mx4_check(__func__, x_codes, x_scales, M, K)) return rc;
     if (int rc = mx4_check(__func__, w_codes, w_scales, N, K)) return rc;
     if (int rc = mx4_check_product(__func__, x_codes, K, y_dtype, K, bias, bias_dtype, y, ldy, N, M)) return rc;
-    if (int rc = mx4_check_tiles(__func__, M, N, K)) return rc;
+    if (int rc = mx4_check_tiles(__func__, M, N, K, mx4_product_tile(M, N))) return rc;
     if (int rc = mx4_check_workspace(__func__, workspace, workspace_bytes, drm_mx4_product_workspace_bytes(M, N, K))) return rc;
     hipStream_t s = (hipStream_t)stream;
     const Mx4 X{x_codes, x_scales, M, mx4_blocks(K)}, W{w_codes, w_scales, N, mx4_blocks(K)};

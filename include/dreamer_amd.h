@@ -550,7 +550,8 @@ int drm_layer_norm_backward(const void* x, int64_t ldx, const void* dy, int64_t 
  *   loss[r] = sum_j p_j (log p_j - log q_{i_j}) + P (log P - log Q)
  * forward also writes p_out (rows, k) and row_out (rows, 4), which backward takes; `workspace`:
  * drm_distill_topk_workspace_bytes(rows, V) bytes (may be 0).  backward: d_logits (rows, V; dense, the logits' type) =
- * g_rows[r] * d loss[r] / d logits.  An index that is listed more than once counts with each of its p_j. */
+ * g_rows[r] * d loss[r] / d logits.  An index that is listed more than once counts with each of its p_j.
+ * rows * ceil(V / 4096) may be up to 2^31 - 1 (DRM_ENOTSUP beyond). */
 size_t drm_distill_topk_workspace_bytes(int64_t rows, int32_t V);
 int drm_distill_topk_forward(const void* logits, int64_t ld_logits, int32_t dtype, const float* top_values, int64_t ld_values,
                              const int64_t* top_indices, int64_t ld_indices, const float* top_lse, int64_t rows, int32_t V, int32_t k,
@@ -570,7 +571,8 @@ int drm_distill_topk_backward(const void* logits, int64_t ld_logits, int32_t dty
  *               are exact (x in bf16 parts on the bf16 matrix pipe), sums are fp32.
  *   dgrad     : dx (M, K) = dy W, the input gradient of `linear`.
  *   product   : y (M, N) = X W^T + bias with both operands in 4 bits (scaled matrix instructions), y of y_dtype.
- * Products take up to 8388480 rows and reductions of up to 4194304 elements (DRM_ENOTSUP beyond). */
+ * Products take up to 8388480 rows, reductions of up to 4194304 elements and, above 32 rows (and in dgrad and product), fewer than
+ * 2^23 tiles of 128 x 128 outputs (product: 256 x 256 where there are so many) (DRM_ENOTSUP beyond). */
 int drm_mx4_quantize(const void* x, int64_t ldx, int32_t dtype, int64_t rows, int32_t K, uint8_t* codes, uint8_t* scales,
                      drm_stream_t stream);
 int drm_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int32_t K, void* y, int64_t ldy, int32_t dtype,

@@ -72,3 +72,55 @@ def test_a_product_of_4_bit_rows_has_its_bias_gradient(rows, dtype, bias_dtype):
     assert torch.equal(plain, y.detach()) and not plain.requires_grad and not mx4.linear(a, w).requires_grad
     with forward_ad.dual_level(), pytest.raises(NotImplementedError):
         mx4.linear(a, w, forward_ad.make_dual(b.detach(), torch.ones(40, device=DEV, dtype=bias_dtype)))
+
+
+# A launch takes fewer than 2^32 threads along an axis: one workgroup per row, or per tile of a weight's rows, reaches that.
+def test_distillation_of_more_rows_than_one_grid_axis_takes():
+    part, times, V = 1021, 65731, 2                  # 2^26 rows and some of 64 threads each; every row repeats one of 1021
+    g = torch.Generator(device=DEV).manual_seed(1)
+    s, values = torch.randn(part, V, generator=g, device=DEV).to(F16), torch.randn(part, 1, generator=g, device=DEV)
+    idx = torch.randint(-1, V, (part, 1), generator=g, device=DEV)
+    lse = values.flatten() + 0.5
+    dy = torch.rand(part, generator=g, device=DEV)
+    few = s.clone().requires_grad_()
+    want = losses.distill_topk_rows(few, values, idx, 1.0, lse)
+    (want_grad,) = torch.autograd.grad(want, few, dy)
+    many = s.repeat(times, 1).requires_grad_()
+    assert many.shape[0] > 2 ** 26
+    got = losses.distill_topk_rows(many, values.repeat(times, 1), idx.repeat(times, 1), 1.0, lse.repeat(times))
+    (grad,) = torch.autograd.grad(got, many, dy.repeat(times))
+    assert bool((got.detach().view(times, part) == want.detach()).all()) and bool((grad.view(times, part, V) == want_grad).all())
+
+
+@pytest.mark.parametrize("K,rows", [(30, 2 ** 27 + 40), (32, 2 ** 29 + 100)])
+def test_few_rows_and_a_weight_of_more_rows_than_one_grid_axis_takes(K, rows):
+    part = 3 * 2 ** 12 - 4                           # (no multiple of a workgroup's weight rows)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    w = mx4.quantize(torch.randn(part, K, generator=g, device=DEV))
+    x = torch.randn(1, K, generator=g, device=DEV).to(BF16)
+    times = -(-rows // part)
+    codes, scales = (t.repeat(times, 1)[:rows] for t in (w.codes, w.scales))
+    y = mx4.linear(x, mx4.MX4Tensor(codes, scales, K))
+    del codes, scales
+    # a sum of K <= 32 exact products in another order (another kernel may serve the short weight), rounded once
+    ref = x.double() @ w.dequantize().double().t()
+    tol = 2.0 ** -8 * ref.abs() + (K + 2) * U * (x.double().abs() @ w.dequantize().double().abs().t())
+    whole = rows // part
+    body = y[:, :whole * part].view(whole, part)
+    assert bool((body == body[0]).all()) and bool((y[0, whole * part:] == body[0, :rows - whole * part]).all())
+    assert float(((body[:1].double() - ref).abs() - tol).max()) <= 0
+
+
+def test_column_sums_of_rows_longer_than_one_grid_axis_takes():
+    E = 2 ** 26 + 3                                  # 2 E sums, joined 32 a workgroup of 1024 threads
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(1, E, generator=g, device=DEV)
+    w, b = torch.ones(E, device=DEV, requires_grad=True), torch.zeros(E, device=DEV, requires_grad=True)
+    dy = torch.randn(1, E, generator=g, device=DEV)
+    y = norm.layer_norm(x, w, b)
+    dw, db = torch.autograd.grad(y, (w, b), dy)
+    assert torch.equal(db, dy[0])                    # one row: its own gradient
+    # dw = dy xh, and y = xh: one product, of two factors that are each the kernel's own to a few half steps (xh is formed as
+    # (x - m) r in both passes: a difference, a product, and a fused step with w = 1, b = 0)
+    want = dy[0].double() * y.detach()[0].double()
+    assert float(((dw.double() - want).abs() - 8 * U * want.abs()).max()) <= 0

@@ -42,3 +42,13 @@ def test_layer_norm_takes_weight_and_bias_of_one_type():
             norm.layer_norm(x, w, b)
     for w, b in ((one, one), (one.bfloat16(), one.bfloat16()), (one, None), (None, one.bfloat16())):
         assert norm.layer_norm(x, w, b).dtype == torch.bfloat16
+
+
+def test_products_of_too_many_tiles_are_refused():
+    """A launch takes fewer than 2^32 threads along an axis, 512 of them a tile of 128 x 128 outputs."""
+    L, P, big = N.lib(), 1 << 20, 1 << 60
+    for M, rows in ((33, 2 ** 30), (33, 2 ** 31 - 300), (128 * 65535, 128 * 129)):
+        rc = L.drm_mx4_linear(P, 32, 1, P, P, None, 0, P, rows, M, rows, 32, P, big, None)
+        assert rc == -95 and "too many tiles" in L.drm_last_error().decode()
+    rc = L.drm_mx4_product(P, P, P, P, None, 0, P, 2 ** 30, 1, 128 * 65535, 2 ** 30, 32, P, big, None)
+    assert rc == -95 and "too many tiles" in L.drm_last_error().decode()
