@@ -412,13 +412,13 @@ __global__ __launch_bounds__(256) void k_observe_st_bwd(const StBwdArgs P) {
     }
 }
 
-// defined in imagine.hip's translation unit as well; both are file-local
-// (a kernel rather than a memset: callers record this pass into graphs, where memset nodes have gone wrong on later replays)
+// a kernel rather than a memset: callers record this pass into graphs, where memset nodes have gone wrong on later replays
 __global__ __launch_bounds__(256) void k_zero_o(float* __restrict__ p, int64_t n) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i < n) p[i] = 0.f;
 }
 
+// defined in imagine.hip's translation unit as well; both are file-local
 __global__ __launch_bounds__(256) void k_transpose_cols_o(const float* __restrict__ W, int64_t ldw, int col0, int ncols,
                                                            int nrows, float* __restrict__ out) {
     __shared__ float tile[32][33];
