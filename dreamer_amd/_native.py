@@ -816,7 +816,9 @@ def wants_grad(a, b=None, c=None) -> bool:
     the values and drop the tangent."""
     if torch.is_grad_enabled() and (a.requires_grad or (b is not None and b.requires_grad) or (c is not None and c.requires_grad)):
         return True
-    return in_dual_level() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (a, b, c))
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (a, b, c))
 
 
 def layer_norm_forward(x, weight, bias, eps: float, want_stats: bool):
