@@ -12,14 +12,19 @@
 // them.  Forward keeps a running maximum and sum per thread over groups of slots (one rescaling per group), backward is one
 // multiplication of exp((s - m) / T) by a factor per row.  With the teacher's log-sum-exp the unlisted entries are summed by
 // themselves (a bitmap of the listed ones in LDS): log Q = -log1p(listed / unlisted) keeps its digits where Q is close to 1,
-// and so does log P = log1p(-sum p).  Sums run in 32 bits per thread and in 64 bits across threads; the per-row scalars are
-// formed in 64 bits because they are small differences of numbers close to 1.
+// and so does log P = log1p(-sum p).  The per-row scalars are formed in 64 bits because they are small differences of numbers
+// close to 1.  Held in 32 bits, each for half a step or a few of a sum of positive terms (the loss is off by 6e-8 at 240 x 255):
+// a thread's sum of exponentials (its terms come from a 32-bit exponential); the sums of a segment on their way to the join (a row
+// of one segment keeps its 64 bits across threads); 1 / T as the exponent's factor, see exp_scaled; and p, which backward
+// subtracts from a 32-bit q.
 //
 // A row is cut into segments, one workgroup each: with one segment the row is finished in the same launch, else a second kernel
 // joins the segments' (maximum, sum).
-// 4096 x 32768 bf16, 64 listed: forward 50 us (5.4 TB/s), with the rest 58 to 65 us (the masks; the exponentials of a row take
+// 4096 x 32768 bf16, 64 listed: forward 51 us (5.3 TB/s), with the rest 59 us (the masks; the exponentials of a row take
 // half of its time), backward 95 us (5.7 TB/s).  Rows of a few thousand logits are bound by the end of a row: two logarithms and
-// up to three exponentials in 64 bits by one wave, about 1.5 us of a SIMD (65536 x 1024: 96 us, with the rest 152 us, 1.4 and 0.9 TB/s).
+// up to three exponentials in 64 bits, about 1.5 us of a SIMD because a wave ends one row and its lanes form the same scalars
+// (65536 x 1024: 89 us, with the rest 140 us, 1.7 and 1.1 TB/s, where the bytes alone would take 32 us).
+// Times here and below: recorded graph of twenty calls in a row, per call.
 #include "elem.hpp"
 
 #include <algorithm>
@@ -28,8 +33,8 @@
 
 namespace drm {
 
-constexpr int DISTILL_SEG = 32768;     // entries a workgroup takes forward (a bitmap of 4 KiB): 4096 x 32768 with the rest 58 us (16384: 65, 8192: 70), 16 x 131072 15 us (13, 11)
-constexpr int DISTILL_SEG_BWD = 4096;  // and backward, where nothing has to be joined: 4096 x 32768 bf16 95 us (16384: 113, 32768: 120), 16 x 32768 3.6 us (5.5, 8.2)
+constexpr int DISTILL_SEG = 32768;     // entries a workgroup takes forward (a bitmap of 4 KiB): 4096 x 32768 with the rest 59 us (16384: 65, 8192: 70), 16 x 131072 15 us (13, 11)
+constexpr int DISTILL_SEG_BWD = 4096;  // and backward, where nothing has to be joined: 4096 x 32768 bf16 95 us (16384: 113, 32768: 120), 16 x 32768 3.4 us (5.5, 8.2)
 constexpr int DISTILL_MAX_K = 1024;
 
 struct DistillRow {                    // what backward needs of a row (both factors 0: no gradient)
@@ -389,8 +394,8 @@ extern "C" int drm_distill_topk_forward(const void* logits, int64_t ld_logits, i
     ProfScope ps(PC_ELEMENTWISE, s, 6 * n, n * elem_bytes(dtype) + (double)rows * k * 12);
     return with_elem(dtype, [&](auto tag) -> int {
         using T = decltype(tag);
-        // one wave a row: more rows under way (8192 x 4096 bf16 21 us, four waves a row 34); few longer rows want the four (256 x
-        // 8192: 7.5 and 6.0 us)
+        // one wave a row: more rows under way (8192 x 4096 bf16 22 us, four waves a row 34); few longer rows want the four (256 x
+        // 8192: 7.5 and 5.8 us)
         const int64_t most = launch_limit(V <= 4096 ? 64 : 256) / A.segs;
         for (int64_t r = 0; r < rows; r += most) {
             const DistillArgs P = A.from<T>(r);
@@ -422,7 +427,7 @@ extern "C" int drm_distill_topk_backward(const void* logits, int64_t ld_logits, 
     ProfScope ps(PC_ELEMENTWISE, s, 5 * n, 2 * n * elem_bytes(dtype) + (double)rows * k * 12);
     return with_elem(dtype, [&](auto tag) -> int {
         using T = decltype(tag);
-        // (32768 x 1024 bf16: one wave 35 us, four 46; 1024 x 4096: 6.5 and 5.3)
+        // (32768 x 1024 bf16: one wave 30 us, four 46; 1024 x 4096: 6.5 and 5.3)
         const int64_t most = launch_limit(V <= 2048 ? 64 : 256) / A.segs;
         for (int64_t r = 0; r < rows; r += most) {
             const DistillBwdArgs P = A.from<T>(r);

@@ -9,8 +9,10 @@
 // bias stay in registers for all of them, and so do the column sums of the backward pass, which go to `partials` once per
 // workgroup and are added there in a fixed order (no atomics: results do not depend on the order in which workgroups run).
 // Rates of the bytes that must move, where a copy of 4 GiB reaches 4.7 TB/s (smaller ones stay in part in the caches):
-//   bf16 16384 x 4096  forward 42 us (6.4 TB/s), backward 85 us (4.7);   1048576 x 64  48 us (5.6), 83 us (4.9)
-//   fp32 65536 x 512   forward 41 us (6.5),      backward 82 us (4.9);   4096 x 16384  98 us (5.5), 170 us (4.7)
+//   bf16 16384 x 4096  forward 45 us (5.9 TB/s), backward 80 us (5.0);   1048576 x 64  48 us (5.6), 82 us (4.9)
+//   fp32 65536 x 512   forward 41 us (6.5),      backward 83 us (4.9);   4096 x 16384  98 us (5.5), 168 us (4.8)
+// (recorded graph of twenty calls in a row, per call, as all times in this file; by itself under the profiler a kernel of this size
+// takes up to a tenth more or less: bf16 16384 x 4096 forward 43 us, 4096 x 16384 forward 50 us in a row and 56 us by itself)
 #include "colsum.hpp"
 
 #include <algorithm>
@@ -269,7 +271,7 @@ __global__ __launch_bounds__(256) void k_norm_bwd_narrow(const T* __restrict__ x
 
 // Rows too long for registers: three walks over the row (the second and third find it in the caches unless it is longer than
 // those).  One workgroup per row, four slots under way per thread: at 512 threads they fit the registers (1024 x 65536 bf16
-// 82 us, 3.3 TB/s; at 1024 threads 110 us, spilled).
+// 80 us, 3.4 TB/s; at 1024 threads 110 us, spilled).
 template <typename T, int TPB>
 __global__ __launch_bounds__(TPB) void k_norm_fwd_long(const T* __restrict__ x, int64_t ldx, const void* w, const void* b, int wtype,
                                                        T* __restrict__ y, int64_t ldy, float* __restrict__ mean,
@@ -335,7 +337,7 @@ __global__ __launch_bounds__(TPB <= 64 ? 256 : TPB, 4) void k_norm_bwd(const T* 
                                                                     int E) {
     constexpr int VEC = Elem<T>::VEC, RPB = TPB <= 64 ? 256 / TPB : 1;
     // Sixteen elements at 1024 threads, 128 registers each: the weight is read again for every row, and the column sums stay in
-    // LDS, each thread's its own (4096 x 16384 bf16: 115 us, 3.5 TB/s; all in registers, which spill, 170 us).
+    // LDS, each thread's its own (4096 x 16384 bf16: 116 us, 3.5 TB/s; all in registers, which spill, 170 us).
     constexpr bool KEEP = CH * VEC <= 8, AHEAD = KEEP || sizeof(T) == 2;      // (fp32: no registers left for the next row's)
     static_assert(KEEP || TPB > 64, "column sums in LDS: one row per workgroup");
     using Part = RowPart<T, TPB, CH>;
@@ -460,7 +462,7 @@ __global__ __launch_bounds__(TPB <= 64 ? 256 : TPB, 4) void k_norm_bwd(const T* 
     }
 }
 
-// The long rows backward, x and dy read twice: the two row means first (2048 x 32768 bf16, all three kernels: 149 us) ...
+// The long rows backward, x and dy read twice: the two row means first (2048 x 32768 bf16, all three kernels: 143 us) ...
 template <typename T, int TPB>
 __global__ __launch_bounds__(TPB) void k_norm_bwd_sums(const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy, int64_t lddy,
                                                         const void* w, int wtype, const float* __restrict__ mean,
@@ -571,8 +573,8 @@ __global__ __launch_bounds__(256) void k_norm_bwd_cols(const T* __restrict__ x, 
 // ---- host side -------------------------------------------------------------------------------------------------------
 // Threads per row by the row's length: the fewest lanes whose slots cover it, at most 16 elements a thread forward and 8 backward
 // (x, dy, the next row's, weight, two running column sums: 80 to 100 registers, four to five waves per SIMD).  Forward with 8
-// instead: 65536 x 1024 bf16 47 us against 44, 8192 x 8192 51 against 45; backward with 16 spills or needs the LDS.
-// Forward above 16384: two-byte rows up to 32768 stay in registers with the weight read again (2048 x 32768: 79 us, three
+// instead: 65536 x 1024 bf16 47 us against 41, 8192 x 8192 51 against 46; backward with 16 spills or needs the LDS.
+// Forward above 16384: two-byte rows up to 32768 stay in registers with the weight read again (2048 x 32768: 75 us, three
 // walks 88), fp32 rows walk (1024 x 32768: 76 us, in registers 126).
 constexpr int NORM_MAX_E = 1024 * 16;
 template <typename T>
@@ -580,7 +582,7 @@ static constexpr int norm_max_fwd() { return sizeof(T) == 2 ? 2 * NORM_MAX_E : N
 template <typename T>
 static inline bool norm_narrow(int E) { return E < Elem<T>::VEC; }
 // Workgroups that walk the rows backward; each leaves 2 E column sums.  At most about four waves per SIMD (65536 x 1024 bf16: 512
-// workgroups 115 us, 1024 82 us, 2048 88 us; 16384 x 4096: 128 125 us, 256 81 us, 1024 96 us), and of four rows at least where
+// workgroups 115 us, 1024 82 us, 2048 88 us; 16384 x 4096: 128 125 us, 256 80 us, 1024 96 us), and of four rows at least where
 // rows are few (1024 x 1024: 256 workgroups 9 us, one per row 15 us).
 static inline int norm_slices(int64_t N, int E, int x_dtype) {
     if (N < 1) return 1;
@@ -650,7 +652,7 @@ extern "C" int drm_layer_norm_forward(const void* x, int64_t ldx, int32_t x_dtyp
         } else {
             norm_variant<T, false>(E, [&](auto tpb, auto ch) {
                 constexpr int TPB = decltype(tpb)::value, CH = decltype(ch)::value, RPB = TPB <= 64 ? 256 / TPB : 1;
-                // four times the workgroups that the chip holds at once (16384 x 4096 bf16 42 us, once 46 us, sixteen times 48 us);
+                // four times the workgroups that the chip holds at once (16384 x 4096 bf16 side by side 42 us, once 46, sixteen times 48);
                 // of 1024 threads as many as it holds (4096 x 16384: 50 us, four times 64 us)
                 const int64_t groups = (N + RPB - 1) / RPB, cap = TPB <= 64 ? 8192 : 256 * (TPB < 1024 ? 8192 : 2048) / TPB;
                 k_norm_fwd<T, TPB, CH, true><<<(int)(groups < cap ? groups : cap), TPB <= 64 ? 256 : TPB, 0, s>>>((const T*)x, ldx, w, b, w_dtype, (T*)y, ldy, mean, rstd, N, E, eps);

@@ -94,8 +94,9 @@ __device__ const uint4 mx4_zero_block = {0u, 0u, 0u, 0u};
 // reads the fragments there.  A lane holds one block of a weight row and feeds it to four instructions, eight elements at a
 // time; the four lane groups hold different blocks, a permutation of the reduction index that x follows.  x comes from L2 for every
 // workgroup, which is why a wave takes NT weight tiles to one fragment of x.  The waves' sums meet in LDS in a fixed order.
-// Bound by the weight's bytes: 16 x 12288 x 4096 bf16 9.3 us (2.9 TB/s; an empty launch takes 3 us of it), 16 x 8192 x 8192 10.6 us
-// (3.4 TB/s).  fp32 rows have three parts, three times the instructions and the x traffic: 16 x 12288 x 4096 17 us.
+// Bound by the weight's bytes: 16 x 12288 x 4096 bf16 9.4 us (2.9 TB/s; an empty launch takes 3 us of it), 16 x 8192 x 8192 10.5 us
+// (3.4 TB/s).  fp32 rows have three parts, three times the instructions and the x traffic: 16 x 12288 x 4096 17 us
+// (fp16, two parts: 11.5 us).  Times here and below: recorded graph of twenty calls in a row, per call.
 template <typename T, int MT, int NT, int NW>
 struct RowsStage {
     __attribute__((aligned(16))) uint8_t w[NW][NT * 1024], x[NW][MT * 16 * 128 * sizeof(T)];
@@ -316,8 +317,8 @@ __device__ __forceinline__ void mx4_store_tile(float* strip, const f32x16 (&acc)
 //       rows, for one conversion per two elements, at the rate of ordinary vector instructions, under the matrix instructions).
 //   dx: the reduction runs over W's rows, so that a fragment needs one column of eight rows: the block of a row is widened
 //       once, four rows side by side exchange their dwords (a transposition among four lanes), and the columns go to LDS.
-// bf16, y / dx: 1024 x 4096 x 4096 45 / 48 us (765 TFLOP/s; a library product of the same size with a bf16 weight 39 / 45 us),
-// 2048 x 8192 x 4096 153 / 168 us (900).  fp16 rows have two parts (82 / 88 us), fp32 rows three (120 / 120 us).  Bound by the
+// bf16, y / dx: 1024 x 4096 x 4096 42 / 47 us (830 TFLOP/s; a library product of the same size with a bf16 weight 39 / 45 us),
+// 2048 x 8192 x 4096 145 / 161 us (950).  fp16 rows have two parts (81 / 88 us), fp32 rows three (116 / 117 us).  Bound by the
 // issue of vector and LDS instructions between the matrix instructions, which are busy a third of the time.
 constexpr int TILE_WAVES = 8, TILE_THREADS = TILE_WAVES * 64;
 template <typename T, int BK, bool GRAD>
@@ -634,7 +635,8 @@ __global__ __launch_bounds__(TILE_THREADS) void k_mx4_tile(const T* __restrict__
 // An instruction's lane half h takes block 4 h + s of the step's eight in its s-th turn -- a permutation of the reduction index that
 // both operands share -- so that one dword holds a lane's four scales and the turn selects the byte.
 // Blocks behind the last one come from the zero block, rows behind the last one repeat it and are not stored.
-// 8192^3: 290 to 304 us, 3.6 to 3.8 PFLOP/s; 4096^3: 45 to 48 us, 2.9; 1024 x 4096 x 4096: 20 us, 1.7 (tiles of 128).  The instructions alone,
+// 8192^3: 277 to 300 us in a row by the board and what ran before it (3.7 to 4.0 PFLOP/s; single calls under the profiler 282 to 340,
+// 320 at the mean); 4096^3: 42 to 45 us, 3.2; 1024 x 4096 x 4096: 18 us, 1.9 (tiles of 128).  The instructions alone,
 // from registers, reach 8.4 PFLOP/s with zeros but 5.7 to 6.5 with random codes, for which the clock falls (2.4 to below 2.0 GHz):
 // that, not the nominal rate, is the ceiling.  Matrix instructions are busy 45 to 48% of the time; without the loads from memory the
 // same loop takes 255 us, with a quarter of the LDS reads besides 214 us.
@@ -864,7 +866,7 @@ __global__ __launch_bounds__(256) void k_mx4_colsum(const T* __restrict__ dy, in
     }
 }
 // About four workgroups a CU, of 32 rows at least: 2048 x 8192 bf16 6.6 us (5.1 TB/s; 16 slices and one thread for each joined
-// column 17 us), 1024 x 4096 5.1 us (8 rows at least 6.8).
+// column 17 us), 1024 x 4096 4.8 us (8 rows at least 6.8).
 static inline int mx4_colsum_slices(int M, int N) {
     const int64_t want = std::max<int64_t>(1, 1024 / ((N + 255ll) / 256));
     return (int)std::min<int64_t>(std::min<int64_t>(want, 256), (M + 31ll) / 32);
@@ -906,8 +908,8 @@ static inline size_t mx4_part_bytes(int slices, int M, int N) { return slices > 
 static inline int mx4_step_of(int dtype) { return dtype == DRM_BF16 ? 128 : 64; }
 
 // Large products: bf16 rows whose 16-byte chunks are aligned and whole go to LDS by direct loads with 128 of the reduction per step
-// (1024 x 4096 x 4096 45.6 us, through registers 50.0; 2048 x 8192 x 4096 153 and 166), in three stages where a row's scales are
-// whole dwords (two: 46.2 and 156 us); through registers the parts of wider types leave room for 64.
+// (side by side: 1024 x 4096 x 4096 45.6 us, through registers 50.0; 2048 x 8192 x 4096 153 and 166), in three stages where a row's
+// scales are whole dwords (two: 46.2 and 156 us); through registers the parts of wider types leave room for 64.
 template <bool GRAD, typename T>
 static void mx4_launch_tile(const T* x, int64_t ldx, const Mx4& W, const void* bias, int btype, T* y, int64_t ldy, int M, int N, int K,
                             float* part, hipStream_t s) {

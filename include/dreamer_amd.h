@@ -531,7 +531,8 @@ int drm_ln_silu_backward(const float* x, const float* dy, const float* gamma, co
  *   forward : y (N, E; row stride ldy) = (x - mean) * rstd * w + b; mean, rstd (N, fp32) are written when not NULL (both or
  *             neither).
  *   backward: dx (N, E; dense, x_dtype), dw, db (E; w_dtype), each of them optional.  dw and db are summed over the rows through
- *             `workspace` (drm_layer_norm_workspace_bytes(N, E)) in an order that depends on N and E only.
+ *             `workspace` (drm_layer_norm_workspace_bytes(N, E)) in an order that depends on N, E and
+ *             x_dtype only.
  * N = 0 is allowed (dw = db = 0). */
 int drm_layer_norm_forward(const void* x, int64_t ldx, int32_t x_dtype, const void* w, const void* b, int32_t w_dtype, void* y,
                            int64_t ldy, float* mean, float* rstd, int64_t N, int32_t E, float eps, drm_stream_t stream);
