@@ -1,4 +1,6 @@
 """What the layer norm, distillation and 4-bit operators promise beyond their values, on the device."""
+import threading
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -25,7 +27,7 @@ def test_forward_mode_derivatives_are_refused():
         calls = [lambda: norm.layer_norm(dual(x), w, b), lambda: norm.layer_norm(x, dual(w), b), lambda: norm.layer_norm(x, None, dual(b)),
                  lambda: norm.layer_norm(dual(x).view(2, 2, 64)), lambda: mx4.linear(dual(x), q), lambda: mx4.linear(x, q, dual(b4)),
                  lambda: losses.distill_topk_rows(dual(x), values, idx)]
-        for n, call in enumerate(calls):
+        for call in calls:
             with pytest.raises(NotImplementedError):
                 call()
             with torch.no_grad(), pytest.raises(NotImplementedError):
@@ -72,6 +74,70 @@ def test_a_product_of_4_bit_rows_has_its_bias_gradient(rows, dtype, bias_dtype):
     assert torch.equal(plain, y.detach()) and not plain.requires_grad and not mx4.linear(a, w).requires_grad
     with forward_ad.dual_level(), pytest.raises(NotImplementedError):
         mx4.linear(a, w, forward_ad.make_dual(b.detach(), torch.ones(40, device=DEV, dtype=bias_dtype)))
+
+
+def test_on_another_stream_and_in_a_recorded_graph():
+    """The product of two 4-bit matrices with the gradient of its bias."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x, w = torch.randn(70, 4096, generator=g, device=DEV), mx4.quantize(torch.randn(200, 4096, generator=g, device=DEV))
+    b = torch.randn(200, generator=g, device=DEV)
+
+    def step(rows, bias):
+        bias = bias.detach().requires_grad_()                 # a leaf of its own
+        y = mx4.linear(mx4.quantize(rows), w, bias)
+        return [y.detach(), *torch.autograd.grad((y * rows[:, :200]).sum(), bias)]
+
+    eager = step(x, b)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = step(x, b)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(p, q) for p, q in zip(eager, other))
+    xs, bs = x.clone(), b.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(xs, bs)
+    for n in range(3):
+        xs.copy_(x * (n + 1))
+        bs.copy_(b - n)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, step(xs.clone(), bs.clone())))
+
+
+def test_two_threads_on_streams_of_their_own():
+    """Nothing is shared between calls: two threads, each on its stream with tensors of its own, get what one gets."""
+    w = mx4.quantize(torch.randn(300, 2048, device=DEV))
+
+    def step(x, values, idx):
+        leaf = x.clone().requires_grad_()
+        y = mx4.linear(norm.layer_norm(leaf), w)
+        z = mx4.linear(mx4.quantize(leaf), w)
+        loss = losses.distill_topk_rows(y, values, idx, 2.0)
+        return [y.detach(), z, loss.detach(), torch.autograd.grad(loss.sum(), leaf)[0]]
+
+    work = []
+    for n in range(2):
+        x = torch.randn(50 + 30 * n, 2048, device=DEV)
+        work.append((x, *torch.randn(x.shape[0], 300, device=DEV).topk(7, 1)))
+    want = [step(*job) for job in work]
+    torch.cuda.synchronize()
+    wrong = [None, None]
+
+    def run(n):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                wrong[n] = [i for i in range(40) if not all(torch.equal(p, q) for p, q in zip(step(*work[n]), want[n]))]
+        except Exception as e:                                # (a thread's exception does not reach the test by itself)
+            wrong[n] = e
+
+    threads = [threading.Thread(target=run, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == [[], []]
 
 
 # A launch takes fewer than 2^32 threads along an axis: one workgroup per row, or per tile of a weight's rows, reaches that.
