@@ -1,10 +1,10 @@
 #!/bin/bash
 # kernel trace and counters of the large cases of tools/operators_times.py:
-#   bash tools/prof_operators.sh        (results under gpurun_out/pops)
+#   bash tools/prof_operators.sh <folder for the results, new>
 set -e
 root=$(pwd)
-out=$root/gpurun_out/pops
-rm -rf "$out"; mkdir -p "$out"
+mkdir "$1"
+out=$(cd "$1" && pwd)
 cd /tmp
 export TMPDIR=/tmp
 run="python3 $root/tools/operators_times.py --calls"
